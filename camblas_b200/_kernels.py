@@ -728,3 +728,324 @@ def reduce_groups(grouped, experts, reverse):
                         grouped.shape[0] * grouped.shape[1], _pointer(experts), _pointer(reverse),
                         _pointer(grouped), _pointer(out))
     return out
+
+
+# ---- the decoding step between the projections ----
+
+
+def _plain_operand(tensor, what):
+    """These operations are for inference; a gradient that was asked for would be lost silently."""
+    _require(not (tensor.requires_grad and torch.is_grad_enabled()),
+             f"{what} requires a gradient: this operation has none, call it under torch.no_grad()")
+
+
+def _strides(*values):
+    return (ct.c_longlong * len(values))(*values)
+
+
+def _heads_operand(tensor, what, reference):
+    """BF16 ``[rows, heads, depth]`` readable in 8-byte pieces where it lies, else a copy."""
+    _require(tensor.is_cuda and tensor.dtype == torch.bfloat16 and tensor.dim() == 3
+             and tensor.device == reference.device, f"{what} must be CUDA BF16 [rows, heads, depth]")
+    _plain_operand(tensor, what)
+    if (tensor.stride(2) != 1 or tensor.stride(0) % 4 or tensor.stride(1) % 4
+            or tensor.data_ptr() % 8):
+        tensor = tensor.clone(memory_format=torch.contiguous_format)
+    return tensor
+
+
+def _cache_type(key_cache, value_cache, reference, kv_heads, depth, alignment):
+    """Check a pair of paged caches and return the type code of the C ABI."""
+    _require(key_cache.is_cuda and key_cache.dim() == 4 and value_cache.dim() == 4
+             and key_cache.shape == value_cache.shape and key_cache.dtype == value_cache.dtype
+             and key_cache.device == reference.device == value_cache.device,
+             "Caches must be two CUDA tensors [pages, page size, kv_heads, depth] of one shape and dtype")
+    _require(key_cache.dtype in (torch.bfloat16, torch.float8_e4m3fn), "Caches are BF16 or FP8 E4M3")
+    _require(key_cache.shape[2] == kv_heads and key_cache.shape[3] == depth
+             and key_cache.shape[1] >= 1 and key_cache.shape[0] <= _INT_MAX
+             and key_cache.shape[1] <= _INT_MAX, "Cache shape does not match the heads")
+    width = key_cache.element_size()
+    for cache in (key_cache, value_cache):
+        _plain_operand(cache, "cache")
+        _require(cache.stride(3) == 1 and cache.data_ptr() % alignment == 0
+                 and all(stride * width % alignment == 0 for stride in cache.stride()[:3]),
+                 f"Caches need unit stride along the depth and {alignment}-byte aligned rows")
+    return 2 if key_cache.dtype == torch.bfloat16 else 3
+
+
+def rotary_table(positions, rotary, base=10000.0, device="cuda"):
+    """Cosines and sines for ``qk_norm_rope``: FP32 ``[positions, rotary]``.
+
+    Row ``p`` holds ``cos(p * base**(-2i/rotary))`` for ``i < rotary/2``, then the
+    sines. The angles are formed in FP64 (in FP32 the angle of position 100 000
+    is off by up to 4e-3) and the results rounded once.
+    """
+    _require(positions >= 0 and rotary >= 0 and rotary % 2 == 0 and base > 0,
+             "rotary_table takes a number of positions, an even width and a positive base")
+    inverse = float(base) ** (-torch.arange(0, rotary, 2, dtype=torch.float64, device=device) / max(rotary, 1))
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inverse
+    return torch.cat((angle.cos(), angle.sin()), dim=1).float()
+
+
+def _rotate(q, k, v, q_weight, k_weight, epsilon, positions, table, interleaved, caches=None, slots=None,
+            key_scale=1.0, value_scale=1.0):
+    q = _heads_operand(q, "q", q)
+    k = _heads_operand(k, "k", q)
+    tokens, heads, depth = q.shape
+    kv_heads = k.shape[1]
+    _require(k.shape[0] == tokens and k.shape[2] == depth and heads >= 1 and kv_heads >= 1
+             and 8 <= depth <= 256 and depth % 8 == 0 and tokens <= _INT_MAX
+             and heads <= 65536 and kv_heads <= 65536,
+             "q and k must be [tokens, heads, depth] with one depth, a multiple of 8 up to 256")
+    for weight in (q_weight, k_weight):
+        if weight is not None:
+            _require(weight.is_cuda and weight.dtype == torch.bfloat16 and weight.device == q.device
+                     and weight.dim() == 1 and weight.shape[0] == depth and weight.is_contiguous()
+                     and weight.data_ptr() % 8 == 0, "Norm weights must be contiguous CUDA BF16 [depth]")
+            _plain_operand(weight, "norm weight")
+    _require(table.is_cuda and table.dtype == torch.float32 and table.dim() == 2
+             and table.device == q.device and table.is_contiguous() and table.shape[0] <= _INT_MAX
+             and table.shape[1] <= depth and table.shape[1] % 8 == 0 and table.data_ptr() % 16 == 0,
+             "table must be contiguous CUDA FP32 [positions, rotary], rotary a multiple of 8 up to the depth")
+    _require(epsilon >= 0, "epsilon must not be negative")
+    indices = (positions,) if slots is None else (positions, slots)
+    for index in indices:
+        _require(index.is_cuda and index.dtype == torch.int64 and index.device == q.device
+                 and index.dim() == 1 and index.shape[0] == tokens and index.is_contiguous(),
+                 "positions and slots must be contiguous CUDA int64, one per token")
+    q_out = torch.empty((tokens, heads, depth), dtype=q.dtype, device=q.device)
+    k_out, code, pages, page_size = None, 0, 0, 1
+    key_cache = value_cache = None
+    if caches is None:
+        k_out = torch.empty((tokens, kv_heads, depth), dtype=q.dtype, device=q.device)
+        strides = _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1))
+    else:
+        v = _heads_operand(v, "v", q)
+        _require(v.shape == k.shape, "v must have the shape of k")
+        key_cache, value_cache = caches
+        code = _cache_type(key_cache, value_cache, q, kv_heads, depth, 4 * key_cache.element_size())
+        _require(key_cache.data_ptr() != value_cache.data_ptr() or key_cache.numel() == 0,
+                 "Keys and values need caches of their own")
+        _require(0 < key_scale < float("inf") and 0 < value_scale < float("inf"),
+                 "Cache scales must be positive and finite")
+        pages, page_size = key_cache.shape[0], key_cache.shape[1]
+        strides = _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                           *key_cache.stride()[:3], *value_cache.stride()[:3])
+    if tokens:
+        with torch.cuda.device(q.device):
+            native = _native.context(q.device.index)
+            native.call("qk_norm_rope", tokens, heads, kv_heads, depth, table.shape[1], int(bool(interleaved)),
+                        float(epsilon), _pointer(q), _pointer(k), _pointer(v), strides, _pointer(q_weight),
+                        _pointer(k_weight), _pointer(positions), _pointer(table), table.shape[0],
+                        _pointer(q_out), _pointer(k_out), code, _pointer(key_cache), _pointer(value_cache),
+                        pages, page_size, float(key_scale), float(value_scale),
+                        _pointer(slots))
+    return q_out, k_out
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, epsilon, positions, table, interleaved=False):
+    """RMS norm of every query and key head, then the position rotation, in one pass.
+
+    ``q`` ``[tokens, heads, depth]`` and ``k`` ``[tokens, kv_heads, depth]`` are BF16 and may be
+    views of a packed projection. ``y = x * rsqrt(mean(x^2) + epsilon) * weight`` over the depth
+    (a weight of ``None``: ``y = x``), then pairs ``(i, i + rotary/2)``, or ``(2i, 2i+1)`` when
+    ``interleaved``, of the first ``rotary = table.shape[1]`` elements turn by the angles whose
+    cosines and sines ``table`` (``rotary_table``) holds for the token's ``positions`` (int64).
+    FP32 throughout, one rounding. Returns contiguous ``(q, k)``; a token whose position is
+    outside the table is padding and gives zeros.
+    """
+    return _rotate(q, k, None, q_weight, k_weight, epsilon, positions, table, interleaved)
+
+
+def qk_norm_rope_append(q, k, v, q_weight, k_weight, epsilon, positions, table, key_cache, value_cache,
+                        slots, key_scale=1.0, value_scale=1.0, interleaved=False):
+    """``qk_norm_rope`` whose keys, with the values ``v``, go straight into a paged cache.
+
+    The caches are ``[pages, page size, kv_heads, depth]`` BF16 or FP8 E4M3 in any order of
+    strides with unit stride along the depth. Token ``i`` is written to slot ``slots[i]`` (int64,
+    ``page * page_size + place``); a slot outside the cache, or a position outside the table,
+    writes nothing; slots that are written must be distinct. An E4M3 cache receives
+    ``key / key_scale`` and ``value / value_scale``, rounded once from FP32, at most 448 in
+    magnitude. Returns the new queries.
+    """
+    return _rotate(q, k, v, q_weight, k_weight, epsilon, positions, table, interleaved,
+                   (key_cache, value_cache), slots, key_scale, value_scale)[0]
+
+
+def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, window=0, sinks=0,
+                    key_scale=1.0, value_scale=1.0):
+    """Attention of one new token per sequence over a paged cache, BF16 ``[batch, heads, depth]``.
+
+    ``q`` is BF16 ``[batch, heads, depth]``; the caches are those of ``qk_norm_rope_append``
+    (16-byte aligned rows; E4M3 depths are multiples of 16), ``heads`` a multiple of their
+    ``kv_heads``. Token ``t`` of sequence ``b`` lies at place ``t % page size`` of page
+    ``table[b, t // page size]`` (int32); it is visible when ``t < lengths[b]`` (int32) and, with
+    ``window > 0``, when it is one of the last ``window`` or of the first ``sinks`` tokens. A token
+    whose page number is outside the cache is not visible, a sequence that sees nothing gives
+    zeros. The default scale is ``1 / sqrt(depth)``. The work is cut over the lengths found on the
+    device, so a captured call follows them; the same call gives the same bits.
+    """
+    q = _heads_operand(q, "q", q)
+    batch, heads, depth = q.shape
+    _require(key_cache.dim() == 4, "Caches must be [pages, page size, kv_heads, depth]")
+    kv_heads = key_cache.shape[2]
+    code = _cache_type(key_cache, value_cache, q, kv_heads, depth, 16)
+    _require(heads >= 1 and kv_heads >= 1 and heads % kv_heads == 0 and heads <= 65536
+             and batch * heads <= _INT_MAX and 8 <= depth <= 256 and depth % (16 if code == 3 else 8) == 0,
+             "paged_attention takes heads a multiple of kv_heads and a depth of a multiple of 8 (E4M3: 16) up to 256")
+    _require(table.is_cuda and table.dtype == torch.int32 and table.device == q.device and table.dim() == 2
+             and table.shape[0] == batch and table.shape[1] <= _INT_MAX
+             and (table.shape[1] <= 1 or table.stride(1) == 1) and table.stride(0) >= 0,
+             "table must be CUDA int32 [batch, pages of a sequence] with unit column stride")
+    _require(lengths.is_cuda and lengths.dtype == torch.int32 and lengths.device == q.device
+             and lengths.dim() == 1 and lengths.shape[0] == batch and lengths.is_contiguous(),
+             "lengths must be contiguous CUDA int32 [batch]")
+    _require(0 <= window <= _INT_MAX and 0 <= sinks <= _INT_MAX, "window and sinks must not be negative")
+    if scale is None:
+        scale = depth ** -0.5
+    out = torch.empty((batch, heads, depth), dtype=q.dtype, device=q.device)
+    if batch:
+        with torch.cuda.device(q.device):
+            native = _native.context(q.device.index)
+            size = _native.library().camblas_cuda_paged_attention_workspace(
+                native.handle, batch, heads, kv_heads, depth, code, key_cache.shape[1], table.shape[1],
+                window, sinks)
+            # of the calling stream's pool, or of the capturing graph's own: no other call shares it
+            workspace = torch.empty((size,), dtype=torch.uint8, device=q.device)
+            native.call("paged_attention", batch, heads, kv_heads, depth, float(scale), _pointer(q), code,
+                        _pointer(key_cache), _pointer(value_cache),
+                        _strides(q.stride(0), q.stride(1), *key_cache.stride()[:3], *value_cache.stride()[:3],
+                                 table.stride(0)),
+                        key_cache.shape[0], key_cache.shape[1], float(key_scale), float(value_scale),
+                        _pointer(table), table.shape[1], _pointer(lengths), window, sinks,
+                        _pointer(workspace), size, _pointer(out))
+    return out
+
+
+class Int4Weight:
+    """A 4-bit weight with group scales, laid out once for ``int4_linear``.
+
+    ``codes`` is uint8 ``[outputs, inner/2]``, two codes per byte, low nibble first; ``scale``
+    BF16 or FP32 ``[outputs, inner/group]`` with groups of 32, 64 or 128 inputs; ``zero`` uint8
+    0..15 of the same shape, or ``None`` for 8 throughout. Element ``(o, k)`` stands for
+    ``(code - zero) * scale``. The codes are copied into the order the kernel's lanes read
+    (``camblas_cuda_int4_linear``), outputs padded to 16 and inputs to 64; the arguments are not
+    kept.
+    """
+
+    def __init__(self, codes, scale, zero=None):
+        _require(codes.is_cuda and codes.dtype == torch.uint8 and codes.dim() == 2 and codes.shape[0] >= 1
+                 and codes.shape[1] >= 16, "codes must be CUDA uint8 [outputs, inner/2]")
+        outputs, inner = codes.shape[0], 2 * codes.shape[1]
+        _require(scale.device == codes.device and scale.dtype in (torch.bfloat16, torch.float32)
+                 and scale.dim() == 2 and scale.shape[0] == outputs and scale.shape[1] >= 1
+                 and inner % scale.shape[1] == 0 and inner // scale.shape[1] in (32, 64, 128),
+                 "scale must be BF16 or FP32 [outputs, inner/group] with groups of 32, 64 or 128")
+        _require(outputs <= _INT_MAX - 16 and inner <= _INT_MAX - 64, "LP64 dimension overflow")
+        self.outputs, self.inner, self.group = outputs, inner, inner // scale.shape[1]
+        tiles, blocks = (outputs + 15) // 16, (inner + 63) // 64
+
+        def tiled(values):  # [outputs, groups] -> [tile, group, g, r], padded with zeros
+            padded = torch.zeros((tiles * 16, values.shape[1]), dtype=values.dtype, device=values.device)
+            padded[:outputs] = values
+            return padded.view(tiles, 2, 8, -1).permute(0, 3, 2, 1).contiguous()
+
+        if zero is not None:
+            _require(zero.device == codes.device and zero.dtype == torch.uint8 and zero.shape == scale.shape
+                     and int(zero.max()) <= 15, "zero must be uint8 0..15 of the shape of scale")
+            zero = tiled(zero)
+        self.scale, self.zero = tiled(scale.detach()), zero
+        words = torch.zeros((tiles, blocks, 8, 4, 2, 2), dtype=torch.int32, device=codes.device)
+        padded = torch.zeros((tiles * 16, blocks * 32), dtype=torch.uint8, device=codes.device)
+        padded[:outputs, :inner // 2] = codes
+        # [tile, r, g, block, h, t, m, j // 2], a byte holding j % 2 = 0 (low nibble) and 1
+        parts = padded.view(tiles, 2, 8, blocks, 2, 4, 2, 2)
+        for r in range(2):
+            for pair in range(2):
+                byte = parts[:, r, ..., pair].permute(0, 2, 1, 4, 3, 5).int()  # [tile, block, g, t, h, m]
+                at = 4 * (r + 2 * pair)
+                words |= ((byte & 15) << at) | ((byte >> 4) << (at + 16))
+        self.codes = words
+
+
+def int4_linear(x, weight, bias=None, residual=None):
+    """``x @ W.T (+ bias) (+ residual)`` for a 4-bit ``Int4Weight``, BF16 ``[..., outputs]``.
+
+    The products are of exact operands (whole numbers against BF16), sums and scales FP32, with
+    one rounding. Made for the few token rows of decoding, where reading the weight is the cost:
+    up to 32 rows read it once, more rows once per 32.
+    """
+    _require(isinstance(weight, Int4Weight), "weight must be an Int4Weight")
+    _check_tensor(x, x)
+    _plain_operand(x, "x")
+    _require(x.dim() >= 1 and x.shape[-1] == weight.inner and x.device == weight.codes.device,
+             "int4_linear requires x [..., inner] on the weight's device")
+    inner, outputs = weight.inner, weight.outputs
+    rows = x.numel() // inner
+    _require(rows <= 65535, "int4_linear takes at most 65535 rows")
+    x2 = x.reshape(rows, inner)
+    if x2.stride(-1) != 1 or (rows > 1 and (x2.stride(0) < inner or x2.stride(0) % 8)) or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    if bias is not None:
+        _check_tensor(bias, x, "bias")
+        _plain_operand(bias, "bias")
+        _require(bias.dim() == 1 and bias.shape[0] == outputs and bias.is_contiguous(),
+                 "linear bias must have the output width")
+    r2 = None
+    if residual is not None:
+        _check_tensor(residual, x, "residual")
+        _plain_operand(residual, "residual")
+        _require(tuple(residual.shape) == tuple(x.shape[:-1]) + (outputs,), "residual must have the output shape")
+        r2 = residual.reshape(rows, outputs)
+        if r2.stride(-1) != 1 or (rows > 1 and r2.stride(0) < outputs):
+            r2 = r2.contiguous()
+    out = torch.empty((rows, outputs), dtype=x.dtype, device=x.device)
+    if rows:
+        with torch.cuda.device(x.device):
+            native = _native.context(x.device.index)
+            native.call("int4_linear", rows, inner, outputs, weight.group, _pointer(x2),
+                        x2.stride(0) if rows > 1 else inner, _pointer(weight.codes),
+                        0 if weight.scale.dtype == torch.float32 else 2, _pointer(weight.scale),
+                        _pointer(weight.zero), _pointer(bias), _pointer(r2),
+                        (r2.stride(0) if rows > 1 else outputs) if r2 is not None else 0,
+                        _pointer(out), outputs)
+    return out.reshape(tuple(x.shape[:-1]) + (outputs,))
+
+
+def route_experts(logits, choices, bias=None, scoring="softmax", groups=1, kept_groups=1, renormalise=True,
+                  scale=1.0):
+    """Choose the experts of every token: ``(ids, weights)``, int64 and FP32 ``[tokens, choices]``.
+
+    ``logits`` is FP32 or BF16 ``[tokens, experts]``. Scores are the softmax over a token's
+    experts or, with ``scoring="sigmoid"``, the sigmoid of each; experts are ranked by score plus
+    ``bias`` (FP32 ``[experts]``). With ``groups > 1`` the experts lie in that many equal groups
+    and only the ``kept_groups`` groups with the largest sum of their two largest ranks are
+    chosen from. ``ids`` are in descending order of rank, equal ranks in ascending order of id
+    (compared in FP64; a NaN ranks last); ``weights`` are the scores, divided by their sum over
+    the chosen when ``renormalise``, times ``scale``. ``ids`` is what ``route_groups`` and
+    ``reduce_groups`` take, ``weights`` the ``routing`` of ``swiglu``.
+    """
+    _require(logits.is_cuda and logits.dim() == 2, "logits must be CUDA [tokens, experts]")
+    _require(logits.dtype in (torch.float32, torch.bfloat16), "logits must be FP32 or BF16")
+    _plain_operand(logits, "logits")
+    tokens, experts = logits.shape
+    _require(scoring in ("softmax", "sigmoid"), "scoring is softmax or sigmoid")
+    _require(tokens <= _INT_MAX and 1 <= experts <= 1024 and 1 <= groups <= 32 and experts % groups == 0
+             and 1 <= kept_groups <= groups and 1 <= choices <= min(32, kept_groups * (experts // groups)),
+             "route_experts takes up to 1024 experts in up to 32 equal groups and up to 32 choices among the kept")
+    if bias is not None:
+        _require(bias.is_cuda and bias.device == logits.device and bias.dtype == torch.float32 and bias.dim() == 1
+                 and bias.shape[0] == experts and bias.is_contiguous(), "bias must be contiguous FP32 [experts]")
+        _plain_operand(bias, "bias")
+    if logits.stride(1) != 1 or (tokens > 1 and logits.stride(0) < experts):
+        logits = logits.contiguous()
+    ids = torch.empty((tokens, choices), dtype=torch.int64, device=logits.device)
+    weights = torch.empty((tokens, choices), dtype=torch.float32, device=logits.device)
+    if tokens:
+        with torch.cuda.device(logits.device):
+            native = _native.context(logits.device.index)
+            native.call("route_experts", 0 if logits.dtype == torch.float32 else 2, tokens, experts, choices,
+                        int(scoring == "sigmoid"), groups, kept_groups, int(bool(renormalise)), float(scale),
+                        _pointer(logits), logits.stride(0) if tokens > 1 else experts, _pointer(bias),
+                        _pointer(ids), _pointer(weights))
+    return ids, weights

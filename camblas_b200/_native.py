@@ -114,6 +114,26 @@ _SIGNATURES = {
     "grouped_quantized_matmul": ([_P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P], _I),
     "route_groups": ([_P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P], _I),
     "reduce_groups": ([_P, _I, _I, _I, _I, _P, _P, _P, _P], _I),
+    "qk_norm_rope": (
+        [_P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _P,
+         ct.c_longlong, _I, _F, _F, _P],
+        _I,
+    ),
+    "paged_attention_workspace": ([_P] + [_I] * 9, ct.c_size_t),
+    "paged_attention": (
+        [_P, _I, _I, _I, _I, _F, _P, _I, _P, _P, _P, _I, _I, _F, _F, _P, _I, _P, _I, _I, _P,
+         ct.c_size_t, _P],
+        _I,
+    ),
+    "int4_linear": (
+        [_P, _I, _I, _I, _I, _P, ct.c_longlong, _P, _I, _P, _P, _P, _P, ct.c_longlong, _P,
+         ct.c_longlong],
+        _I,
+    ),
+    "route_experts": (
+        [_P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, ct.c_longlong, _P, _P, _P],
+        _I,
+    ),
 }
 
 EXPORTED = tuple("camblas_cuda_" + name for name in _SIGNATURES)

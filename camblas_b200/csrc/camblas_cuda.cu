@@ -11,6 +11,10 @@
 #include "fp8_block_wide.cuh"
 #include "gemm_simt.cuh"
 #include "dense_fp.cuh"
+#include "expert_scores.cuh"
+#include "head_rotate.cuh"
+#include "int4_linear.cuh"
+#include "paged_attention.cuh"
 #include "quantized.cuh"
 #include "rms_norm.cuh"
 #include "row_parallel.cuh"
@@ -107,7 +111,7 @@ int create_here(int device, void *stream, camblas_cuda_context **out)
     if (status == 0) {
         what = "kernel attributes";
         status = host::prepare_kernels() | fp8::prepare_kernels() | fp8::prepare_wide_kernels() |
-                 prepare_rms_kernels();
+                 prepare_rms_kernels() | attend::prepare_kernels();
     }
     if (status != 0) {
         cudaGetLastError();

@@ -460,6 +460,111 @@ int camblas_cuda_reduce_groups(camblas_cuda_context *context, int tokens, int ch
                                int grouped_rows, const void *experts, const void *reverse,
                                const void *input, void *output);
 
+/* ---- the decoding step between the projections ---------------------------- */
+
+/* None of the following has a counterpart in the reference ABI, whose attention
+ * is dense, single-head and cacheless (camblas_cuda.h:80-85) and whose expert
+ * routing starts from ids (routing.cuh). A cache holds the keys (and another
+ * the values) of all sequences in pages: [pages][page_size][kv_heads][depth],
+ * any strides but unit stride along depth, cache_type 2 BF16 or 3 E4M3. An E4M3
+ * entry stands for value = entry * scale, with one scale for the keys and one
+ * for the values. */
+
+/* RMS norm of every query and key head with its weight, then the position
+ * rotation, with one rounding:
+ *   y = x * rsqrt(mean(x^2) + epsilon) * weight[depth]   (weight NULL: y = x)
+ *   (a, b) -> (a cos - b sin, b cos + a sin) over the first `rotary` elements,
+ * pairs (i, i + rotary/2), or (2i, 2i+1) when interleaved. q is [tokens, heads,
+ * depth], k and v [tokens, kv_heads, depth] BF16 with unit stride along depth,
+ * weights BF16 [depth], positions int64 [tokens]; table is FP32 [table_rows,
+ * rotary], cosines then sines of a position's rotary/2 angles. A token whose
+ * position is outside the table is padding: its outputs are zero and nothing of
+ * it enters the cache. q_out is [tokens, heads, depth] contiguous.
+ * cache_type 0: k_out [tokens, kv_heads, depth] contiguous; v, slots and the
+ * cache arguments are ignored. cache_type 2 or 3: keys and values go to slot
+ * slots[token] (int64; page * page_size + place in the page) of the caches,
+ * keys from the FP32 result divided by key_scale, values divided by
+ * value_scale, saturating at 448 for E4M3 (with cache_type 2 both scales are
+ * ignored); a slot outside [0, pages * page_size) is not written, slots that
+ * are written must be distinct. k_out may then be NULL. strides, in elements:
+ * {q token, q head, k token, k head, v token, v head, key page, key slot, key
+ * head, value page, value slot, value head}, the last eight only with a cache.
+ * depth a multiple of 8 up to 256, rotary a multiple of 8 up to depth; q, k, v,
+ * outputs 8-byte aligned and their strides multiples of 4; table 16-byte
+ * aligned; caches aligned to 4 elements and their strides multiples of 4.
+ * Outputs overlap no input. */
+int camblas_cuda_qk_norm_rope(camblas_cuda_context *context, int tokens, int heads, int kv_heads,
+                              int depth, int rotary, int interleaved, float epsilon, const void *q,
+                              const void *k, const void *v, const long long *strides,
+                              const void *q_weight, const void *k_weight, const void *positions,
+                              const float *table, int table_rows, void *q_out, void *k_out,
+                              int cache_type, void *key_cache, void *value_cache, long long pages,
+                              int page_size, float key_scale, float value_scale, const void *slots);
+
+/* Attention of one new token per sequence over the cache:
+ *   out[b,h] = sum_t softmax_t(scale q[b,h] . key_t) value_t
+ * over tokens t < lengths[b] (int32 [batch]; negative counts as 0, more than
+ * table_width * page_size as that) and, with window > 0, t >= lengths[b] -
+ * window or t < sinks. Query head h reads key head h / (heads / kv_heads). Token
+ * t lies at place t % page_size of page table[b][t / page_size] (int32 [batch,
+ * table_width]); a token whose page is outside [0, pages) is not visible. A head
+ * without a visible token of finite score gives zeros. q is [batch, heads,
+ * depth] BF16, output the same, contiguous. strides, in elements: {q batch, q
+ * head, key page, key slot, key head, value page, value slot, value head, table
+ * row}. depth a multiple of 8 up to 256 (of 16 for E4M3), heads a multiple of
+ * kv_heads; q 8-byte aligned with strides multiples of 4, caches 16-byte
+ * aligned with strides multiples of 16 bytes. workspace: device memory of at
+ * least camblas_cuda_paged_attention_workspace bytes (0 for invalid sizes),
+ * 16-byte aligned, used by this call only until it has run. No atomics: the
+ * same call gives the same bits. Counter slot 6 counts it. */
+size_t camblas_cuda_paged_attention_workspace(const camblas_cuda_context *context, int batch,
+                                              int heads, int kv_heads, int depth, int cache_type,
+                                              int page_size, int table_width, int window, int sinks);
+int camblas_cuda_paged_attention(camblas_cuda_context *context, int batch, int heads, int kv_heads,
+                                 int depth, float scale, const void *q, int cache_type,
+                                 const void *key_cache, const void *value_cache,
+                                 const long long *strides, int pages, int page_size, float key_scale,
+                                 float value_scale, const void *table, int table_width,
+                                 const void *lengths, int window, int sinks, void *workspace,
+                                 size_t workspace_bytes, void *output);
+
+/* Linear layer with 4-bit weights for a few tokens: out[rows,outputs] = x[rows,
+ * inner] . W^T (+ bias) (+ residual), BF16, where W[o,k] = (code - zero) *
+ * scale, code and zero whole numbers 0..15 (zero 8 when zeros is NULL), scale
+ * and zero of output o and group k / group. Products of exact operands, FP32
+ * sums, scales applied in FP32, one rounding. scale_type 0 FP32, 2 BF16. codes,
+ * scales and zeros in the order that the Int4Weight class of the Python layer
+ * produces: codes [tiles of 16 outputs][blocks of 64 inputs][32 lanes 4g +
+ * t][4 words 2h + m], word nibble r + 2 (j / 2) + 4 (j % 2) = code of output
+ * 16 tile + g + 8r and input 64 block + 32h + 8t + 4m + j; scales, and zeros
+ * (one byte each), [tiles][inner / group][8 g][2 r]; outputs padded to 16,
+ * inputs to 64, with scale zero. group 32, 64 or 128, inner a multiple of it;
+ * rows <= 65535; x 16-byte aligned, ldx a multiple of 8, codes 16-byte aligned.
+ * Above a few dozen rows the weights are read once per 32 rows. */
+int camblas_cuda_int4_linear(camblas_cuda_context *context, int rows, int inner, int outputs,
+                             int group, const void *x, long long ldx, const void *codes,
+                             int scale_type, const void *scales, const void *zeros,
+                             const void *bias, const void *residual, long long ldr, void *out,
+                             long long ldo);
+
+/* Router of a mixture of experts. score = softmax(logits) over a token's
+ * experts, or 1 / (1 + exp(-logits)) when sigmoid; rank = score + bias
+ * (FP32 [experts], NULL: 0). With groups > 1 the experts lie in that many equal
+ * groups, a group's rank is the sum of its two largest ranks (its only one when
+ * it has one expert), and the kept_groups groups of largest rank stay. The
+ * `choices` experts of largest rank in them are written to chosen (int64
+ * [tokens, choices]) in descending order; weights (FP32, same shape) = score
+ * (renormalise: / the sum of the chosen scores; 0 where that is 0) * scale.
+ * Equal ranks go to the lower index, a NaN ranks behind every number; ranks are
+ * compared in FP64. A row without an open expert (all logits -inf) has scores
+ * zero. dtype of logits 0 FP32, 2 BF16, row stride ld_logits in elements.
+ * experts <= 1024, choices <= 32 and <= the experts kept, groups <= 32. */
+int camblas_cuda_route_experts(camblas_cuda_context *context, int dtype, int tokens, int experts,
+                               int choices, int sigmoid, int groups, int kept_groups,
+                               int renormalise, float scale, const void *logits,
+                               long long ld_logits, const float *bias, void *chosen,
+                               float *weights);
+
 /* ---- FP32 / FP64 GEMM ----------------------------------------------------- */
 
 /* Replace camblas_cuda_sgemm / camblas_cuda_dgemm (camblas_cuda.h:57-62;
