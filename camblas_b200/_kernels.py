@@ -733,44 +733,52 @@ def reduce_groups(grouped, experts, reverse):
 # ---- the decoding step between the projections ----
 
 
-def _plain_operand(tensor, what):
+# A call of these takes a few microseconds on the GPU, so the host side counts: devices are
+# compared by index (-1 off the GPU), addresses go to the C ABI as integers, and the current
+# device is left alone (every entry point works on its context's device).
+
+
+def _refuse_gradient(*tensors):
     """These operations are for inference; a gradient that was asked for would be lost silently."""
-    _require(not (tensor.requires_grad and torch.is_grad_enabled()),
-             f"{what} requires a gradient: this operation has none, call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for tensor in tensors:
+            _require(tensor is None or not tensor.requires_grad,
+                     "An operand requires a gradient: this operation has none, call it under torch.no_grad()")
 
 
-def _strides(*values):
-    return (ct.c_longlong * len(values))(*values)
+def _address(tensor):
+    return None if tensor is None else tensor.data_ptr()
 
 
-def _heads_operand(tensor, what, reference):
-    """BF16 ``[rows, heads, depth]`` readable in 8-byte pieces where it lies, else a copy."""
-    _require(tensor.is_cuda and tensor.dtype == torch.bfloat16 and tensor.dim() == 3
-             and tensor.device == reference.device, f"{what} must be CUDA BF16 [rows, heads, depth]")
-    _plain_operand(tensor, what)
-    if (tensor.stride(2) != 1 or tensor.stride(0) % 4 or tensor.stride(1) % 4
-            or tensor.data_ptr() % 8):
+def _heads_operand(tensor, index):
+    """BF16 ``[rows, heads, depth]`` readable in 8-byte pieces where it lies, else a copy; with its
+    row and head strides."""
+    _require(index >= 0 and tensor.get_device() == index and tensor.dtype is torch.bfloat16
+             and tensor.dim() == 3, "Heads must be CUDA BF16 [rows, heads, depth] on one device")
+    row, head, unit = tensor.stride()
+    if unit != 1 or row % 4 or head % 4 or tensor.data_ptr() % 8:
         tensor = tensor.clone(memory_format=torch.contiguous_format)
-    return tensor
+        row, head, unit = tensor.stride()
+    return tensor, row, head
 
 
-def _cache_type(key_cache, value_cache, reference, kv_heads, depth, alignment):
-    """Check a pair of paged caches and return the type code of the C ABI."""
-    _require(key_cache.is_cuda and key_cache.dim() == 4 and value_cache.dim() == 4
-             and key_cache.shape == value_cache.shape and key_cache.dtype == value_cache.dtype
-             and key_cache.device == reference.device == value_cache.device,
-             "Caches must be two CUDA tensors [pages, page size, kv_heads, depth] of one shape and dtype")
-    _require(key_cache.dtype in (torch.bfloat16, torch.float8_e4m3fn), "Caches are BF16 or FP8 E4M3")
-    _require(key_cache.shape[2] == kv_heads and key_cache.shape[3] == depth
-             and key_cache.shape[1] >= 1 and key_cache.shape[0] <= _INT_MAX
-             and key_cache.shape[1] <= _INT_MAX, "Cache shape does not match the heads")
-    width = key_cache.element_size()
-    for cache in (key_cache, value_cache):
-        _plain_operand(cache, "cache")
-        _require(cache.stride(3) == 1 and cache.data_ptr() % alignment == 0
-                 and all(stride * width % alignment == 0 for stride in cache.stride()[:3]),
-                 f"Caches need unit stride along the depth and {alignment}-byte aligned rows")
-    return 2 if key_cache.dtype == torch.bfloat16 else 3
+def _check_caches(key_cache, value_cache, index, kv_heads, depth, alignment):
+    """Check a pair of paged caches; return the type code of the C ABI and their six strides."""
+    kind = key_cache.dtype
+    _require((kind is torch.bfloat16 or kind is torch.float8_e4m3fn) and value_cache.dtype is kind
+             and key_cache.get_device() == index and value_cache.get_device() == index,
+             "Caches must be two CUDA tensors on the device of q, both BF16 or both FP8 E4M3")
+    shape = key_cache.shape
+    _require(len(shape) == 4 and value_cache.shape == shape and shape[2] == kv_heads and shape[3] == depth
+             and shape[1] >= 1 and shape[0] <= _INT_MAX and shape[1] <= _INT_MAX,
+             "Caches must be [pages, page size, kv_heads, depth] of one shape that matches the heads")
+    k0, k1, k2, k3 = key_cache.stride()
+    v0, v1, v2, v3 = value_cache.stride()
+    elements = alignment // (2 if kind is torch.bfloat16 else 1) - 1  # a power of two less one
+    _require(k3 == 1 and v3 == 1 and not (k0 | k1 | k2 | v0 | v1 | v2) & elements
+             and not (key_cache.data_ptr() | value_cache.data_ptr()) & (alignment - 1),
+             "Caches need unit stride along the depth and aligned rows (16 bytes to read, 4 elements to append)")
+    return (2 if kind is torch.bfloat16 else 3), (k0, k1, k2, v0, v1, v2)
 
 
 def rotary_table(positions, rotary, base=10000.0, device="cuda"):
@@ -787,59 +795,55 @@ def rotary_table(positions, rotary, base=10000.0, device="cuda"):
     return torch.cat((angle.cos(), angle.sin()), dim=1).float()
 
 
-def _rotate(q, k, v, q_weight, k_weight, epsilon, positions, table, interleaved, caches=None, slots=None,
-            key_scale=1.0, value_scale=1.0):
-    q = _heads_operand(q, "q", q)
-    k = _heads_operand(k, "k", q)
+def _rotate(q, k, v, q_weight, k_weight, epsilon, positions, table, interleaved, key_cache=None,
+            value_cache=None, slots=None, key_scale=1.0, value_scale=1.0):
+    _refuse_gradient(q, k, v, q_weight, k_weight, table, key_cache, value_cache)
+    index = q.get_device()
+    q, q_row, q_head = _heads_operand(q, index)
+    k, k_row, k_head = _heads_operand(k, index)
     tokens, heads, depth = q.shape
     kv_heads = k.shape[1]
-    _require(k.shape[0] == tokens and k.shape[2] == depth and heads >= 1 and kv_heads >= 1
-             and 8 <= depth <= 256 and depth % 8 == 0 and tokens <= _INT_MAX
-             and heads <= 65536 and kv_heads <= 65536,
+    _require(k.shape[0] == tokens and k.shape[2] == depth and 8 <= depth <= 256 and depth % 8 == 0
+             and 1 <= heads <= 65536 and 1 <= kv_heads <= 65536 and tokens <= _INT_MAX,
              "q and k must be [tokens, heads, depth] with one depth, a multiple of 8 up to 256")
     for weight in (q_weight, k_weight):
-        if weight is not None:
-            _require(weight.is_cuda and weight.dtype == torch.bfloat16 and weight.device == q.device
-                     and weight.dim() == 1 and weight.shape[0] == depth and weight.is_contiguous()
-                     and weight.data_ptr() % 8 == 0, "Norm weights must be contiguous CUDA BF16 [depth]")
-            _plain_operand(weight, "norm weight")
-    _require(table.is_cuda and table.dtype == torch.float32 and table.dim() == 2
-             and table.device == q.device and table.is_contiguous() and table.shape[0] <= _INT_MAX
-             and table.shape[1] <= depth and table.shape[1] % 8 == 0 and table.data_ptr() % 16 == 0,
-             "table must be contiguous CUDA FP32 [positions, rotary], rotary a multiple of 8 up to the depth")
-    _require(epsilon >= 0, "epsilon must not be negative")
-    indices = (positions,) if slots is None else (positions, slots)
-    for index in indices:
-        _require(index.is_cuda and index.dtype == torch.int64 and index.device == q.device
-                 and index.dim() == 1 and index.shape[0] == tokens and index.is_contiguous(),
-                 "positions and slots must be contiguous CUDA int64, one per token")
-    q_out = torch.empty((tokens, heads, depth), dtype=q.dtype, device=q.device)
-    k_out, code, pages, page_size = None, 0, 0, 1
-    key_cache = value_cache = None
-    if caches is None:
-        k_out = torch.empty((tokens, kv_heads, depth), dtype=q.dtype, device=q.device)
-        strides = _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1))
+        _require(weight is None or (weight.get_device() == index and weight.dtype is torch.bfloat16
+                                    and weight.shape == (depth,) and weight.stride(0) == 1
+                                    and not weight.data_ptr() & 7),
+                 "Norm weights must be contiguous CUDA BF16 [depth]")
+    _require(table.get_device() == index and table.dtype is torch.float32 and table.dim() == 2
+             and table.is_contiguous() and not table.data_ptr() & 15, "table must be contiguous CUDA FP32")
+    rows, rotary = table.shape
+    _require(rows <= _INT_MAX and rotary <= depth and rotary % 8 == 0,
+             "table must be [positions, rotary], rotary a multiple of 8 up to the depth")
+    _require(0 <= epsilon < float("inf"), "epsilon must be finite and not negative")
+    _require(positions.get_device() == index and positions.dtype is torch.int64
+             and positions.shape == (tokens,) and positions.is_contiguous(),
+             "positions must be contiguous CUDA int64, one per token")
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out, code, pages, page_size, strides = None, 0, 0, 1, (q_row, q_head, k_row, k_head)
+    if key_cache is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
-        v = _heads_operand(v, "v", q)
+        v, v_row, v_head = _heads_operand(v, index)
         _require(v.shape == k.shape, "v must have the shape of k")
-        key_cache, value_cache = caches
-        code = _cache_type(key_cache, value_cache, q, kv_heads, depth, 4 * key_cache.element_size())
+        code, cache_strides = _check_caches(key_cache, value_cache, index, kv_heads, depth,
+                                            8 if key_cache.dtype is torch.bfloat16 else 4)
+        _require(slots.get_device() == index and slots.dtype is torch.int64 and slots.shape == (tokens,)
+                 and slots.is_contiguous(), "slots must be contiguous CUDA int64, one per token")
         _require(key_cache.data_ptr() != value_cache.data_ptr() or key_cache.numel() == 0,
                  "Keys and values need caches of their own")
         _require(0 < key_scale < float("inf") and 0 < value_scale < float("inf"),
                  "Cache scales must be positive and finite")
         pages, page_size = key_cache.shape[0], key_cache.shape[1]
-        strides = _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                           *key_cache.stride()[:3], *value_cache.stride()[:3])
+        strides += (v_row, v_head) + cache_strides
     if tokens:
-        with torch.cuda.device(q.device):
-            native = _native.context(q.device.index)
-            native.call("qk_norm_rope", tokens, heads, kv_heads, depth, table.shape[1], int(bool(interleaved)),
-                        float(epsilon), _pointer(q), _pointer(k), _pointer(v), strides, _pointer(q_weight),
-                        _pointer(k_weight), _pointer(positions), _pointer(table), table.shape[0],
-                        _pointer(q_out), _pointer(k_out), code, _pointer(key_cache), _pointer(value_cache),
-                        pages, page_size, float(key_scale), float(value_scale),
-                        _pointer(slots))
+        _native.context(index).call(
+            "qk_norm_rope", tokens, heads, kv_heads, depth, rotary, 1 if interleaved else 0, epsilon,
+            q.data_ptr(), k.data_ptr(), _address(v), (ct.c_longlong * len(strides))(*strides),
+            _address(q_weight), _address(k_weight), positions.data_ptr(), table.data_ptr(), rows,
+            q_out.data_ptr(), _address(k_out), code, _address(key_cache), _address(value_cache), pages,
+            page_size, key_scale, value_scale, _address(slots))
     return q_out, k_out
 
 
@@ -868,8 +872,8 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, epsilon, positions, table, 
     ``key / key_scale`` and ``value / value_scale``, rounded once from FP32, at most 448 in
     magnitude. Returns the new queries.
     """
-    return _rotate(q, k, v, q_weight, k_weight, epsilon, positions, table, interleaved,
-                   (key_cache, value_cache), slots, key_scale, value_scale)[0]
+    return _rotate(q, k, v, q_weight, k_weight, epsilon, positions, table, interleaved, key_cache,
+                   value_cache, slots, key_scale, value_scale)[0]
 
 
 def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, window=0, sinks=0,
@@ -885,40 +889,36 @@ def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, windo
     zeros. The default scale is ``1 / sqrt(depth)``. The work is cut over the lengths found on the
     device, so a captured call follows them; the same call gives the same bits.
     """
-    q = _heads_operand(q, "q", q)
+    _refuse_gradient(q, key_cache, value_cache)
+    index = q.get_device()
+    q, q_row, q_head = _heads_operand(q, index)
     batch, heads, depth = q.shape
     _require(key_cache.dim() == 4, "Caches must be [pages, page size, kv_heads, depth]")
-    kv_heads = key_cache.shape[2]
-    code = _cache_type(key_cache, value_cache, q, kv_heads, depth, 16)
-    _require(heads >= 1 and kv_heads >= 1 and heads % kv_heads == 0 and heads <= 65536
-             and batch * heads <= _INT_MAX and 8 <= depth <= 256 and depth % (16 if code == 3 else 8) == 0,
+    pages, page_size, kv_heads, _ = key_cache.shape
+    code, cache_strides = _check_caches(key_cache, value_cache, index, kv_heads, depth, 16)
+    _require(kv_heads >= 1 and 1 <= heads <= 65536 and heads % kv_heads == 0 and batch * heads <= _INT_MAX
+             and 8 <= depth <= 256 and depth % (16 if code == 3 else 8) == 0,
              "paged_attention takes heads a multiple of kv_heads and a depth of a multiple of 8 (E4M3: 16) up to 256")
-    _require(table.is_cuda and table.dtype == torch.int32 and table.device == q.device and table.dim() == 2
-             and table.shape[0] == batch and table.shape[1] <= _INT_MAX
-             and (table.shape[1] <= 1 or table.stride(1) == 1) and table.stride(0) >= 0,
-             "table must be CUDA int32 [batch, pages of a sequence] with unit column stride")
-    _require(lengths.is_cuda and lengths.dtype == torch.int32 and lengths.device == q.device
-             and lengths.dim() == 1 and lengths.shape[0] == batch and lengths.is_contiguous(),
-             "lengths must be contiguous CUDA int32 [batch]")
+    _require(table.get_device() == index and table.dtype is torch.int32 and table.dim() == 2
+             and table.shape[0] == batch, "table must be CUDA int32 [batch, pages of a sequence]")
+    width = table.shape[1]
+    row, column = table.stride()
+    _require(width <= _INT_MAX and row >= 0 and (width <= 1 or column == 1), "table needs unit column stride")
+    _require(lengths.get_device() == index and lengths.dtype is torch.int32 and lengths.shape == (batch,)
+             and lengths.is_contiguous(), "lengths must be contiguous CUDA int32 [batch]")
     _require(0 <= window <= _INT_MAX and 0 <= sinks <= _INT_MAX, "window and sinks must not be negative")
-    if scale is None:
-        scale = depth ** -0.5
-    out = torch.empty((batch, heads, depth), dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if batch:
-        with torch.cuda.device(q.device):
-            native = _native.context(q.device.index)
-            size = _native.library().camblas_cuda_paged_attention_workspace(
-                native.handle, batch, heads, kv_heads, depth, code, key_cache.shape[1], table.shape[1],
-                window, sinks)
-            # of the calling stream's pool, or of the capturing graph's own: no other call shares it
-            workspace = torch.empty((size,), dtype=torch.uint8, device=q.device)
-            native.call("paged_attention", batch, heads, kv_heads, depth, float(scale), _pointer(q), code,
-                        _pointer(key_cache), _pointer(value_cache),
-                        _strides(q.stride(0), q.stride(1), *key_cache.stride()[:3], *value_cache.stride()[:3],
-                                 table.stride(0)),
-                        key_cache.shape[0], key_cache.shape[1], float(key_scale), float(value_scale),
-                        _pointer(table), table.shape[1], _pointer(lengths), window, sinks,
-                        _pointer(workspace), size, _pointer(out))
+        native = _native.context(index)
+        size = native.workspace_bytes("paged_attention", batch, heads, kv_heads, depth, code, page_size, width,
+                                      window, sinks)
+        # of the calling stream's pool, or of the capturing graph's own: no other call shares it
+        workspace = q.new_empty((size // 2,))
+        strides = (ct.c_longlong * 9)(q_row, q_head, *cache_strides, row)
+        native.call("paged_attention", batch, heads, kv_heads, depth, depth ** -0.5 if scale is None else scale,
+                    q.data_ptr(), code, key_cache.data_ptr(), value_cache.data_ptr(), strides, pages, page_size,
+                    key_scale, value_scale, table.data_ptr(), width, lengths.data_ptr(), window, sinks,
+                    workspace.data_ptr(), size, out.data_ptr())
     return out
 
 
@@ -955,6 +955,7 @@ class Int4Weight:
                      and int(zero.max()) <= 15, "zero must be uint8 0..15 of the shape of scale")
             zero = tiled(zero)
         self.scale, self.zero = tiled(scale.detach()), zero
+        self.scale_type = 0 if scale.dtype == torch.float32 else 2
         words = torch.zeros((tiles, blocks, 8, 4, 2, 2), dtype=torch.int32, device=codes.device)
         padded = torch.zeros((tiles * 16, blocks * 32), dtype=torch.uint8, device=codes.device)
         padded[:outputs, :inner // 2] = codes
@@ -976,40 +977,36 @@ def int4_linear(x, weight, bias=None, residual=None):
     up to 32 rows read it once, more rows once per 32.
     """
     _require(isinstance(weight, Int4Weight), "weight must be an Int4Weight")
-    _check_tensor(x, x)
-    _plain_operand(x, "x")
-    _require(x.dim() >= 1 and x.shape[-1] == weight.inner and x.device == weight.codes.device,
-             "int4_linear requires x [..., inner] on the weight's device")
-    inner, outputs = weight.inner, weight.outputs
+    _refuse_gradient(x, bias, residual)
+    inner, outputs, index = weight.inner, weight.outputs, weight.codes.get_device()
+    _require(x.get_device() == index and x.dtype is torch.bfloat16 and x.dim() >= 1 and x.shape[-1] == inner,
+             "int4_linear requires CUDA BF16 x [..., inner] on the weight's device")
+    lead = x.shape[:-1]
     rows = x.numel() // inner
     _require(rows <= 65535, "int4_linear takes at most 65535 rows")
-    x2 = x.reshape(rows, inner)
-    if x2.stride(-1) != 1 or (rows > 1 and (x2.stride(0) < inner or x2.stride(0) % 8)) or x2.data_ptr() % 16:
+    x2 = x if x.dim() == 2 else x.reshape(rows, inner)
+    ldx, unit = x2.stride()
+    if unit != 1 or (rows > 1 and (ldx < inner or ldx % 8)) or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
+        ldx = inner
+    r2, ldr = None, 0
     if bias is not None:
-        _check_tensor(bias, x, "bias")
-        _plain_operand(bias, "bias")
-        _require(bias.dim() == 1 and bias.shape[0] == outputs and bias.is_contiguous(),
-                 "linear bias must have the output width")
-    r2 = None
+        _require(bias.get_device() == index and bias.dtype is torch.bfloat16 and bias.shape == (outputs,)
+                 and bias.is_contiguous(), "linear bias must be contiguous CUDA BF16 of the output width")
     if residual is not None:
-        _check_tensor(residual, x, "residual")
-        _plain_operand(residual, "residual")
-        _require(tuple(residual.shape) == tuple(x.shape[:-1]) + (outputs,), "residual must have the output shape")
+        _require(residual.get_device() == index and residual.dtype is torch.bfloat16
+                 and residual.shape == (*lead, outputs), "residual must be CUDA BF16 of the output shape")
         r2 = residual.reshape(rows, outputs)
         if r2.stride(-1) != 1 or (rows > 1 and r2.stride(0) < outputs):
             r2 = r2.contiguous()
-    out = torch.empty((rows, outputs), dtype=x.dtype, device=x.device)
+        ldr = r2.stride(0) if rows > 1 else outputs
+    out = x.new_empty((*lead, outputs))
     if rows:
-        with torch.cuda.device(x.device):
-            native = _native.context(x.device.index)
-            native.call("int4_linear", rows, inner, outputs, weight.group, _pointer(x2),
-                        x2.stride(0) if rows > 1 else inner, _pointer(weight.codes),
-                        0 if weight.scale.dtype == torch.float32 else 2, _pointer(weight.scale),
-                        _pointer(weight.zero), _pointer(bias), _pointer(r2),
-                        (r2.stride(0) if rows > 1 else outputs) if r2 is not None else 0,
-                        _pointer(out), outputs)
-    return out.reshape(tuple(x.shape[:-1]) + (outputs,))
+        _native.context(index).call(
+            "int4_linear", rows, inner, outputs, weight.group, x2.data_ptr(), ldx if rows > 1 else inner,
+            weight.codes.data_ptr(), weight.scale_type, weight.scale.data_ptr(), _address(weight.zero),
+            _address(bias), _address(r2), ldr, out.data_ptr(), outputs)
+    return out
 
 
 def route_experts(logits, choices, bias=None, scoring="softmax", groups=1, kept_groups=1, renormalise=True,
@@ -1025,27 +1022,26 @@ def route_experts(logits, choices, bias=None, scoring="softmax", groups=1, kept_
     the chosen when ``renormalise``, times ``scale``. ``ids`` is what ``route_groups`` and
     ``reduce_groups`` take, ``weights`` the ``routing`` of ``swiglu``.
     """
-    _require(logits.is_cuda and logits.dim() == 2, "logits must be CUDA [tokens, experts]")
-    _require(logits.dtype in (torch.float32, torch.bfloat16), "logits must be FP32 or BF16")
-    _plain_operand(logits, "logits")
+    _refuse_gradient(logits, bias)
+    index, dtype = logits.get_device(), logits.dtype
+    _require(index >= 0 and logits.dim() == 2 and (dtype is torch.float32 or dtype is torch.bfloat16),
+             "logits must be CUDA FP32 or BF16 [tokens, experts]")
+    _require(scoring == "softmax" or scoring == "sigmoid", "scoring is softmax or sigmoid")
     tokens, experts = logits.shape
-    _require(scoring in ("softmax", "sigmoid"), "scoring is softmax or sigmoid")
     _require(tokens <= _INT_MAX and 1 <= experts <= 1024 and 1 <= groups <= 32 and experts % groups == 0
-             and 1 <= kept_groups <= groups and 1 <= choices <= min(32, kept_groups * (experts // groups)),
+             and 1 <= kept_groups <= groups and 1 <= choices <= 32 and choices <= kept_groups * (experts // groups),
              "route_experts takes up to 1024 experts in up to 32 equal groups and up to 32 choices among the kept")
-    if bias is not None:
-        _require(bias.is_cuda and bias.device == logits.device and bias.dtype == torch.float32 and bias.dim() == 1
-                 and bias.shape[0] == experts and bias.is_contiguous(), "bias must be contiguous FP32 [experts]")
-        _plain_operand(bias, "bias")
-    if logits.stride(1) != 1 or (tokens > 1 and logits.stride(0) < experts):
+    _require(bias is None or (bias.get_device() == index and bias.dtype is torch.float32 and bias.shape == (experts,)
+                              and bias.is_contiguous()), "bias must be contiguous CUDA FP32 [experts]")
+    row, unit = logits.stride()
+    if unit != 1 or (tokens > 1 and row < experts):
         logits = logits.contiguous()
-    ids = torch.empty((tokens, choices), dtype=torch.int64, device=logits.device)
-    weights = torch.empty((tokens, choices), dtype=torch.float32, device=logits.device)
+        row = experts
+    ids = logits.new_empty((tokens, choices), dtype=torch.int64)
+    weights = logits.new_empty((tokens, choices), dtype=torch.float32)
     if tokens:
-        with torch.cuda.device(logits.device):
-            native = _native.context(logits.device.index)
-            native.call("route_experts", 0 if logits.dtype == torch.float32 else 2, tokens, experts, choices,
-                        int(scoring == "sigmoid"), groups, kept_groups, int(bool(renormalise)), float(scale),
-                        _pointer(logits), logits.stride(0) if tokens > 1 else experts, _pointer(bias),
-                        _pointer(ids), _pointer(weights))
+        _native.context(index).call(
+            "route_experts", 0 if dtype is torch.float32 else 2, tokens, experts, choices,
+            1 if scoring == "sigmoid" else 0, groups, kept_groups, 1 if renormalise else 0, scale,
+            logits.data_ptr(), row if tokens > 1 else experts, _address(bias), ids.data_ptr(), weights.data_ptr())
     return ids, weights

@@ -231,10 +231,14 @@ class Context:
         _check(library().camblas_cuda_create(device, stream, ct.byref(self.handle)), None)
         # what the native side currently holds, so that unchanged settings cost nothing
         self._sent = {"policy": "auto", "family": "auto"}
+        # the selection that was adopted last, so that an unchanged one costs one comparison
+        self._adopted = None
+        self._workspaces = {}
         _REGISTRY.add(self)
 
     def _forward(self, key, value, entry, argument):
         if self._sent.get(key) != value:
+            self._adopted = None
             _check(getattr(library(), "camblas_cuda_" + entry)(self.handle, *argument), self.handle)
             self._sent[key] = value
 
@@ -252,14 +256,30 @@ class Context:
 
     def adopt(self, selection):
         """Bring the native side in line with the calling thread's selection."""
+        wanted = (selection.policy, selection.family, selection.options)
+        if self._adopted == wanted:
+            return
         self.set_algorithm(selection.policy)
         self.force_kernel(selection.family)
         for name, value in selection.options.items():
             self.set_option(name, value)
+        self._adopted = (selection.policy, selection.family, dict(selection.options))
 
     def call(self, name, *arguments):
         """Call ``camblas_cuda_<name>(handle, *arguments)`` and check its status."""
-        _check(getattr(library(), "camblas_cuda_" + name)(self.handle, *arguments), self.handle)
+        status = getattr(library(), "camblas_cuda_" + name)(self.handle, *arguments)
+        if status:
+            _check(status, self.handle)
+
+    def workspace_bytes(self, name, *sizes):
+        """Bytes that ``camblas_cuda_<name>`` wants for these sizes on this context's device."""
+        key = (name, sizes)
+        found = self._workspaces.get(key)
+        if found is None:
+            if len(self._workspaces) >= 1024:
+                self._workspaces.clear()
+            found = self._workspaces[key] = getattr(library(), f"camblas_cuda_{name}_workspace")(self.handle, *sizes)
+        return found
 
     def counters(self, reset=False):
         """Return the eight launch counters as a tuple (optionally clearing them)."""
@@ -288,6 +308,13 @@ class Context:
         self.handle = _P()
 
 
+def _raw_stream(device):
+    """Address of the device's current stream; the public call makes an object of it first,
+    which takes longer than the rest of a look-up."""
+    lookup = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return lookup(device) if lookup else torch.cuda.current_stream(device).cuda_stream
+
+
 def context(device):
     """Return this thread's context for ``device`` and its current stream.
 
@@ -295,13 +322,14 @@ def context(device):
     being captured (``camblas/_native.py:262-266`` in the reference), and a
     context made before a ``fork`` is refused in the child (``:270-271``).
     """
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = _raw_stream(device)
     native = _SELECTION.contexts.get((device, stream))
     if native is not None and native.pid != os.getpid():
         raise RuntimeError("CUDA contexts cannot be reused after fork; use spawn")
     if native is None or not native.handle:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("Warm up CAMBLAS on this stream before CUDA graph capture")
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Warm up CAMBLAS on this stream before CUDA graph capture")
         native = _SELECTION.contexts[(device, stream)] = Context(device, stream)
     native.adopt(_SELECTION)
     return native

@@ -57,12 +57,16 @@ struct Piece { /* four elements of a head */
     float e[4];
 };
 
-__device__ __forceinline__ Piece load_piece(const __nv_bfloat16 *from)
+__device__ __forceinline__ Piece unpack_piece(const uint2 &raw)
 {
-    const uint2 raw = *reinterpret_cast<const uint2 *>(from);
     const float2 low = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&raw.x));
     const float2 high = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&raw.y));
     return {{low.x, low.y, high.x, high.y}};
+}
+
+__device__ __forceinline__ Piece load_piece(const __nv_bfloat16 *from)
+{
+    return unpack_piece(*reinterpret_cast<const uint2 *>(from));
 }
 
 __device__ __forceinline__ void store_piece(__nv_bfloat16 *to, const Piece &p)

@@ -22,21 +22,25 @@
  * rounded to BF16 (to FP16 over an 8-bit cache), at most half a step relative
  * to each weight, like the operands of any BF16 product.
  *
- * Work split. All (sequence, key head, block of 8 or 16 query heads) items are
- * laid end to end in tiles of 64 visible tokens and cut into equal contiguous
- * ranges, one per CTA, so ragged lengths load every SM alike. Every CTA finds
+ * Work split. A warp works alone. The slots of a sequence (key heads times
+ * blocks of 8 or 16 query heads) are taken in teams of four neighbours, two or
+ * one, whichever divides their number, one warp each, so that the warps of a
+ * team read neighbouring heads of the same tokens at the same time: the rows
+ * they fetch lie side by side in a page. The tiles of all (sequence, team)
+ * items are laid end to end and cut into equal contiguous ranges, one per team
+ * of warps of the grid, so ragged lengths load every SM alike. Every warp finds
  * its range from the lengths on the device: no plan on the host, and a captured
- * call follows the lengths of the replay. A range that covers an item whole
- * writes its result; a piece of an item leaves maximum, sum and unscaled result
- * in the workspace (at most two pieces per CTA, its first and its last), and
+ * call follows the lengths of the replay. An item that one range covers whole is
+ * written at once; a piece of an item leaves maximum, sum and unscaled result
+ * in the workspace (at most two pieces per warp, its first and its last), and
  * attend_join adds the pieces of an item in token order. No atomics: the same
  * call gives the same bits.
  *
- * Each of the four warps of a CTA copies its own 16 tokens of a tile into its
- * own shared-memory ring with cp.async and reads nothing of the others until
- * the segment of an item ends, so the main loop has no barrier. Tokens that are
- * not visible are filled with zeros instead of being read: a weight of zero
- * times a NaN would be NaN.
+ * A warp copies its tiles into its own shared-memory ring with cp.async, the
+ * page numbers one tile further ahead, running on into the next item while the
+ * present one is summed; there is no barrier in the kernel. Tokens that are not
+ * visible are filled with zeros instead of being read: a weight of zero times a
+ * NaN would be NaN.
  */
 #pragma once
 
@@ -46,85 +50,129 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 namespace attend
 {
 
-constexpr int kWarps = 4;
-constexpr int kWarpTokens = 16;
-constexpr int kTile = kWarps * kWarpTokens;
+constexpr int kWarps = 4; /* of a CTA */
 
 struct AttendTask {
-    int batch, heads, kv_heads, group, head_blocks, depth;
-    int page_size, page_shift, pages, table_width; /* page_shift < 0: not a power of two */
+    int batch, heads, group, depth;      /* group: query heads per key head */
+    int head_blocks, team, teams;        /* slots = kv_heads * head_blocks = team * teams */
+    int page_size, page_shift, pages; /* page_shift < 0: not a power of two */
+    int room;                         /* tokens that a row of the table can hold */
     int window, sinks;
+    int tile_shift; /* log2 of the tokens of a tile */
+    int workers; /* teams of warps in the grid */
     long long q_batch, q_head, table_row;
     const __nv_bfloat16 *q;
-    heads::CacheLayout keys, values;
+    heads::CacheLayout keys, values; /* strides in bytes */
     const int32_t *table, *lengths;
     float score_scale; /* scale * key scale * log2(e) */
     float value_scale;
-    __nv_bfloat16 *out; /* [batch, heads, depth] contiguous */
-    float *pieces;      /* [grid][2][head slots][depth], then statistics */
-    float *statistics;  /* [grid][2][head slots][2] */
+    __nv_bfloat16 *out;    /* [batch, heads, depth] contiguous */
+    long long *first_tile; /* [batch + 1]: number of the first tile of a sequence, then the total */
+    float4 *pieces;        /* [2 * warps][column block][depth class / 16][32 lanes] */
+    float2 *statistics;    /* [2 * warps][column block][8 heads]: maximum, sum */
 };
 
-/* Tokens of a sequence that are visible, before bad pages are taken out. */
-__device__ __forceinline__ int visible_tokens(const AttendTask &task, int length)
+/* The visible tokens of one sequence: `seen` of them, numbered from 0; number v
+ * is token v, or v + jump from number jump_at on. */
+struct Visible {
+    int seen, jump_at, jump, tiles;
+};
+
+__device__ __forceinline__ Visible visible(const AttendTask &task, int length)
 {
-    const long long room = (long long)task.table_width * task.page_size;
-    int seen = length < 0 ? 0 : (length < room ? length : int(room));
-    if (task.window > 0 && seen > task.window) {
-        const int rest = seen - task.window;
-        seen = task.window + (task.sinks < rest ? task.sinks : rest);
+    length = max(0, min(length, task.room));
+    Visible v{length, 0, 0, 1};
+    if (task.window > 0 && length > task.window) {
+        const int rest = length - task.window;
+        v.jump_at = task.sinks < rest ? task.sinks : rest;
+        v.seen = task.window + v.jump_at;
+        v.jump = length - v.seen;
     }
-    return seen;
+    /* an empty sequence keeps a tile so that its zeros get written */
+    v.tiles = v.seen ? ((v.seen - 1) >> task.tile_shift) + 1 : 1;
+    return v;
 }
 
-__device__ __forceinline__ int clamped_length(const AttendTask &task, int length)
-{
-    const long long room = (long long)task.table_width * task.page_size;
-    return length < 0 ? 0 : (length < room ? length : int(room));
-}
+/* The range of tiles of a worker: `total` in equal parts, the first ones a tile longer. */
+struct Cut {
+    long long each;
+    long long longer; /* workers with one tile more */
 
-/* Tiles of one item of sequence b; an empty one keeps a tile so that its zeros
- * get written. */
-__device__ __forceinline__ int tiles_of(const AttendTask &task, int b)
-{
-    const int seen = visible_tokens(task, task.lengths[b]);
-    return seen ? (seen - 1) / kTile + 1 : 1;
-}
+    __device__ __forceinline__ Cut(long long total, int workers)
+        : each(total / workers), longer(total % workers)
+    {
+    }
+    __device__ __forceinline__ long long start(int worker) const
+    {
+        return each * worker + (worker < longer ? worker : longer);
+    }
+    __device__ __forceinline__ int owner(long long tile) const
+    {
+        const long long in_longer = longer * (each + 1);
+        return int(tile < in_longer ? tile / (each + 1) : longer + (tile - in_longer) / each);
+    }
+};
 
-/* Called by whole warps. Sum of tiles_of over the batch. */
-__device__ __forceinline__ long long total_tiles(const AttendTask &task)
+/* Called by whole warps: inclusive prefix sum over the lanes. */
+__device__ __forceinline__ long long running_sum(long long mine)
 {
-    long long sum = 0;
-    for (int b = threadIdx.x & 31; b < task.batch; b += 32)
-        sum += tiles_of(task, b);
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int offset = 16; offset > 0; offset /= 2)
-        sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-    return sum * task.kv_heads * task.head_blocks;
+    for (int offset = 1; offset < 32; offset *= 2) {
+        const long long other = __shfl_up_sync(0xffffffffu, mine, offset);
+        if (lane >= offset)
+            mine += other;
+    }
+    return mine;
 }
 
-/* Called by whole warps. The sequence that holds tile `tile` of the whole list
- * and the number of the sequence's first tile. */
+/* Called by whole warps. Tiles of all items; the first warp of the grid leaves
+ * the first tile of every sequence for attend_join. */
+__device__ __forceinline__ long long count_tiles(const AttendTask &task, bool keep)
+{
+    const int lane = threadIdx.x & 31;
+    if (!keep) {
+        long long sum = 0;
+        for (int b = lane; b < task.batch; b += 32)
+            sum += visible(task, task.lengths[b]).tiles;
+#pragma unroll
+        for (int offset = 16; offset > 0; offset /= 2)
+            sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+        return sum * task.teams;
+    }
+    long long before = 0;
+    for (int base = 0; base < task.batch; base += 32) {
+        const bool live = base + lane < task.batch;
+        const long long mine =
+            live ? (long long)task.teams * visible(task, task.lengths[base + lane]).tiles : 0;
+        const long long upto = running_sum(mine);
+        if (live)
+            task.first_tile[base + lane] = before + upto - mine;
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0)
+        task.first_tile[task.batch] = before;
+    return before;
+}
+
+/* Called by whole warps. The sequence that holds tile number `tile` of the whole
+ * list, and the number of the sequence's first tile. */
 __device__ __forceinline__ void locate(const AttendTask &task, long long tile, int &sequence,
                                        long long &first)
 {
     const int lane = threadIdx.x & 31;
-    const long long per = (long long)task.kv_heads * task.head_blocks;
     long long before = 0;
     for (int base = 0; base < task.batch; base += 32) {
-        const long long mine = base + lane < task.batch ? per * tiles_of(task, base + lane) : 0;
-        long long upto = mine;
-#pragma unroll
-        for (int offset = 1; offset < 32; offset *= 2) {
-            const long long other = __shfl_up_sync(0xffffffffu, upto, offset);
-            if (lane >= offset)
-                upto += other;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, base + lane < task.batch &&
-                                                             before + upto > tile);
+        const bool live = base + lane < task.batch;
+        const long long mine =
+            live ? (long long)task.teams * visible(task, task.lengths[base + lane]).tiles : 0;
+        const long long upto = running_sum(mine);
+        const unsigned past = __ballot_sync(0xffffffffu, live && before + upto > tile);
         if (past) {
             const int at = __ffs(past) - 1;
             sequence = base + at;
@@ -133,13 +181,40 @@ __device__ __forceinline__ void locate(const AttendTask &task, long long tile, i
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    sequence = task.batch, first = before;
+    sequence = task.batch - 1, first = before; /* not reached: tile is below the total */
 }
 
-__device__ __forceinline__ long long range_start(long long total, int grid, int cta)
-{
-    return total / grid * cta + total % grid * cta / grid;
-}
+/* A place in a worker's range, for the warp that is number `member` of its team. */
+struct Cursor {
+    int sequence, team, tile;
+    int kv_head, head_block;
+    Visible view;
+
+    __device__ __forceinline__ void enter(const AttendTask &task, int b, int member)
+    {
+        sequence = b;
+        if (b < task.batch)
+            view = visible(task, task.lengths[b]);
+        choose(task, 0, member);
+    }
+    __device__ __forceinline__ void choose(const AttendTask &task, int of_teams, int member)
+    {
+        team = of_teams;
+        const int slot = team * task.team + member;
+        kv_head = task.head_blocks == 1 ? slot : slot / task.head_blocks;
+        head_block = slot - kv_head * task.head_blocks;
+    }
+    __device__ __forceinline__ void advance(const AttendTask &task, int member)
+    {
+        if (++tile < view.tiles)
+            return;
+        tile = 0;
+        if (team + 1 < task.teams)
+            choose(task, team + 1, member);
+        else
+            enter(task, sequence + 1, member);
+    }
+};
 
 /* ---- tensor-core pieces ---- */
 
@@ -199,6 +274,14 @@ template <bool Half> __device__ __forceinline__ uint32_t pack(float low, float h
     }
 }
 
+/* 2^x; 0 for -infinity */
+__device__ __forceinline__ float power_of_two(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 /* two E4M3 values (exact in FP16), the lower byte in the lower half */
 __device__ __forceinline__ uint32_t widen(uint32_t two_bytes)
 {
@@ -207,7 +290,7 @@ __device__ __forceinline__ uint32_t widen(uint32_t two_bytes)
     return uint32_t(pair.x) | (uint32_t(pair.y) << 16);
 }
 
-/* ---- the kernel ---- */
+/* ---- the kernels ---- */
 
 /* Depth: 64, 128 or 256, the stored depth rounded up. Blocks: 8-head column
  * blocks served by one pass over the keys. Eight: 8-bit cache. */
@@ -221,416 +304,514 @@ template <int Depth, int Blocks, bool Eight> struct Shape {
     {
         return 16u * uint32_t(kChunks >= 8 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3));
     }
-    static constexpr int kStageBytes = 2 * kWarpTokens * kRowBytes; /* keys and values */
-    static constexpr int kStages = kStageBytes >= 16384 ? 3 : (kStageBytes >= 8192 ? 3 : 4);
-    static constexpr int kHeads = 8 * Blocks;
-    static constexpr int kJoinPitch = Depth + 4; /* heads two apart fall eight banks apart */
-    static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-    static constexpr int kJoinBytes = kWarps * kHeads * kJoinPitch * 4;
-    static constexpr int kBytes = kRingBytes + kJoinBytes + kWarps * kHeads * 8 + kWarps * kStages * 4;
-    /* CTAs whose shared memory fits an SM: 228 KB, of which each CTA takes 1 KB more than it asks for */
+    static constexpr int kPieces = Depth / 16; /* 16-row products along the depth */
+    /* Tokens of a tile: 8 KB of keys and values where rows are short, so that what a tile costs
+     * beside its products (page numbers, maxima across lanes) is spread over as many bytes. */
+    static constexpr int kTile = kRowBytes >= 256 ? 16 : (kRowBytes == 128 ? 32 : 64);
+    static constexpr int kGroups = kTile / 16; /* of 16 tokens */
+    static constexpr int kTileShift = kTile == 16 ? 4 : (kTile == 32 ? 5 : 6);
+    static constexpr int kTileBytes = 2 * kTile * kRowBytes; /* keys and values */
+    /* The copies in flight on an SM have to cover the latency of HBM at its share of the
+     * bandwidth, some 45 KB. */
+    static constexpr int kStages = 3;
+    static constexpr int kNoteBytes = 16 * kTile + 16; /* where the rows of a stage lie, which are real */
+    static constexpr int kWarpBytes = kStages * (kTileBytes + kNoteBytes);
+    static constexpr int kBytes = kWarps * kWarpBytes;
+    /* CTAs on an SM: shared memory is 228 KB, of which each CTA takes 1 KB more than it asks for */
     static constexpr int kResident = 228 * 1024 / (kBytes + 1024);
+    static_assert(kResident >= 1 && kResident <= 4, "registers");
 };
 
+/* Result of 16 depths and 8 heads, `o` in the accumulator layout (rows g and
+ * g + 8, heads 2t and 2t + 1), times factor[head]: BF16 rows of the heads at
+ * `out`, of which `live` exist. */
+template <bool Eight>
+__device__ __forceinline__ void store_heads(__nv_bfloat16 *out, int depth, int live, int piece,
+                                            const float (&o)[4], const float (&factor)[2])
+{
+    const int lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
+    const uint32_t low = transpose_8x8(pack<false>(o[0] * factor[0], o[1] * factor[1]));
+    const uint32_t high = transpose_8x8(pack<false>(o[2] * factor[0], o[3] * factor[1]));
+    /* now head g, rows 2t and 2t + 1 of the lower and of the upper half */
+    if (g >= live)
+        return;
+    uint32_t *row = reinterpret_cast<uint32_t *>(out + (long long)g * depth);
+    if constexpr (Eight) { /* see the value product of attend_kernel */
+        const int d = 32 * (piece / 2) + 8 * t + 2 * (piece & 1);
+        if (d < depth) {
+            row[d / 2] = __byte_perm(low, high, 0x5410);
+            row[d / 2 + 2] = __byte_perm(low, high, 0x7632);
+        }
+    } else {
+        const int d = 16 * piece + 2 * t;
+        if (d < depth)
+            row[d / 2] = low;
+        if (d + 8 < depth)
+            row[d / 2 + 4] = high;
+    }
+}
+
 template <int Depth, int Blocks, bool Eight>
-__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const AttendTask task)
+__global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kResident)
+    attend_kernel(const __grid_constant__ AttendTask task)
 {
     using S = Shape<Depth, Blocks, Eight>;
     extern __shared__ __align__(128) uint8_t shared[];
-    float *join = reinterpret_cast<float *>(shared + S::kRingBytes);
-    float *join_stats = reinterpret_cast<float *>(shared + S::kRingBytes + S::kJoinBytes);
-    uint32_t *stage_seen = reinterpret_cast<uint32_t *>(join_stats + kWarps * S::kHeads * 2);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int g = lane / 4, t = lane % 4;
-    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(shared)) +
-                          warp * S::kStages * S::kStageBytes;
-    uint32_t *seen_words = stage_seen + warp * S::kStages;
+    const int global_warp = blockIdx.x * kWarps + warp;
+    const int worker = global_warp / task.team, member = global_warp % task.team;
+    /* the ring of this warp, then the notes of its stages: byte offsets of keys and values of the
+     * rows, and the mask of the real ones */
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(shared)) + warp * S::kStages * S::kTileBytes;
+    uint8_t *notes = shared + kWarps * S::kStages * S::kTileBytes + warp * S::kStages * S::kNoteBytes;
 
-    const long long total = total_tiles(task);
-    const long long begin = range_start(total, gridDim.x, blockIdx.x);
-    const long long end = range_start(total, gridDim.x, blockIdx.x + 1);
-    if (begin >= end)
+    const long long total = count_tiles(task, global_warp == 0);
+    const Cut cut(total, task.workers);
+    const long long begin = cut.start(worker);
+    const int count = int(cut.start(worker + 1) - begin);
+    if (count <= 0 || worker >= task.workers)
         return;
-    int sequence;
-    long long sequence_first;
-    locate(task, begin, sequence, sequence_first);
+    Cursor use;
+    {
+        long long first;
+        int sequence;
+        locate(task, begin, sequence, first);
+        use.enter(task, sequence, member);
+        const int item = int((begin - first) / use.view.tiles);
+        use.choose(task, item, member);
+        use.tile = int(begin - first - (long long)item * use.view.tiles);
+    }
+    Cursor ahead = use; /* the tile whose page numbers are fetched next */
+    int fetched = 0;
+    constexpr int kOwn = (S::kTile + 31) / 32; /* rows of a tile that a lane looks up: lane, lane + 32 */
+    int page[kOwn], place_in_page[kOwn], page_head = 0; /* of the tile that is copied next */
 
-    for (long long tile = begin; tile < end;) {
-        /* the item and the segment [from, upto) of its tiles */
-        const int length = clamped_length(task, task.lengths[sequence]);
-        const int seen = visible_tokens(task, length);
-        const int tiles = seen ? (seen - 1) / kTile + 1 : 1;
-        const int item = int((tile - sequence_first) / tiles);
-        const long long item_first = sequence_first + (long long)item * tiles;
-        const int from = int(tile - item_first);
-        const int upto = int(end - item_first < tiles ? end - item_first : tiles);
-        const int kv_head = item / task.head_blocks;
-        const int head_block = item % task.head_blocks;
-        const int first_head = kv_head * task.group + head_block * S::kHeads;
-        const int live_heads = min(S::kHeads, task.group - head_block * S::kHeads);
-        const int jump_at = task.window > 0 && length > task.window ? seen - task.window : 0;
-        const int jump = length - seen; /* tokens between the sinks and the window */
-        const int32_t *table_row = task.table + sequence * task.table_row;
-
-        const auto issue = [&](int j) {
-            const int stage = (j - from) % S::kStages;
-            const uint32_t base = ring + stage * S::kStageBytes;
-            int page = -1, slot = 0;
-            if (lane < kWarpTokens && j < upto) {
-                int v = j * kTile + warp * kWarpTokens + lane;
-                if (v < seen) {
-                    v += v >= jump_at ? jump : 0;
+    const auto fetch = [&] {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            page[i] = -1;
+        if (fetched < count) {
+            page_head = ahead.kv_head;
+            const int32_t *row = task.table + ahead.sequence * task.table_row;
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                int v = ahead.tile * S::kTile + 32 * i + lane;
+                if ((S::kTile >= 32 || lane < S::kTile) && v < ahead.view.seen) {
+                    v += v >= ahead.view.jump_at ? ahead.view.jump : 0;
                     const int number = task.page_shift >= 0 ? v >> task.page_shift : v / task.page_size;
-                    slot = v - number * task.page_size;
-                    page = table_row[number];
-                    if (page < 0 || page >= task.pages)
-                        page = -1;
+                    place_in_page[i] = v - number * task.page_size;
+                    page[i] = row[number];
                 }
             }
-            const uint32_t real = __ballot_sync(0xffffffffu, page >= 0);
+            ahead.advance(task, member);
+        }
+        ++fetched;
+    };
+    const int chunk = lane % S::kChunks, sub = lane / S::kChunks;
+    const bool inside = chunk * 16 < task.depth * (Eight ? 1 : 2);
+    const uint8_t *const key_base = static_cast<const uint8_t *>(task.keys.base) + chunk * 16;
+    const uint8_t *const value_base = static_cast<const uint8_t *>(task.values.base) + chunk * 16;
+    const auto copy = [&](int stage) {
+        uint8_t *note = notes + stage * S::kNoteBytes;
+        uint32_t real[kOwn], any = 0;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const bool real_row = unsigned(page[i]) < unsigned(task.pages);
+            real[i] = __ballot_sync(0xffffffffu, real_row);
+            any |= real[i];
+            if (S::kTile >= 32 || lane < S::kTile) {
+                longlong2 at = make_longlong2(0, 0);
+                if (real_row) {
+                    at.x = page[i] * task.keys.page_stride + place_in_page[i] * task.keys.slot_stride +
+                           page_head * task.keys.head_stride;
+                    at.y = page[i] * task.values.page_stride + place_in_page[i] * task.values.slot_stride +
+                           page_head * task.values.head_stride;
+                }
+                reinterpret_cast<longlong2 *>(note)[32 * i + lane] = at;
+            }
             if (lane == 0)
-                seen_words[stage] = real;
-            if (real) {
-                constexpr int kRows = 32 / S::kChunks; /* rows a warp copies at once */
-                const int chunk = lane % S::kChunks;
-                const bool inside = chunk * 16 < task.depth * (Eight ? 1 : 2);
-                constexpr int kElement = Eight ? 1 : 2;
+                reinterpret_cast<uint32_t *>(note + 16 * S::kTile)[i] = real[i];
+        }
+        __syncwarp();
+        if (any) {
+            constexpr int kRows = 32 / S::kChunks; /* rows the warp copies at once */
+            const uint32_t base = ring + stage * S::kTileBytes + sub * S::kRowBytes;
 #pragma unroll
-                for (int r = 0; r < kWarpTokens; r += kRows) {
-                    const int row = r + lane / S::kChunks;
-                    const int row_page = __shfl_sync(0xffffffffu, page, row);
-                    const int row_slot = __shfl_sync(0xffffffffu, slot, row);
-                    const bool load = row_page >= 0 && inside;
-                    const uint32_t to = base + row * S::kRowBytes + S::place(row, chunk);
-                    const uint8_t *k = static_cast<const uint8_t *>(task.keys.base);
-                    const uint8_t *v = static_cast<const uint8_t *>(task.values.base);
-                    if (load) {
-                        k += (row_page * task.keys.page_stride + row_slot * task.keys.slot_stride +
-                              kv_head * task.keys.head_stride) * kElement + chunk * 16;
-                        v += (row_page * task.values.page_stride + row_slot * task.values.slot_stride +
-                              kv_head * task.values.head_stride) * kElement + chunk * 16;
-                    }
-                    copy_16(to, k, load);
-                    copy_16(to + kWarpTokens * S::kRowBytes, v, load);
-                }
+            for (int r = 0; r < S::kTile; r += kRows) {
+                const longlong2 at = reinterpret_cast<const longlong2 *>(note)[r + sub];
+                const bool load = inside && (real[r / 32] >> (r % 32 + sub)) & 1;
+                const uint32_t to = base + r * S::kRowBytes + S::place(r + sub, chunk);
+                copy_16(to, key_base + at.x, load);
+                copy_16(to + S::kTile * S::kRowBytes, value_base + at.y, load);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        fetch();
+    };
+    fetch();
+#pragma unroll
+    for (int s = 0; s < S::kStages - 1; ++s)
+        copy(s);
 
+    uint32_t qf[Blocks][S::kPieces][2]; /* Q^T as the column operand: lane (g, t) holds head g */
+    float head_scale[Blocks][2];        /* of heads 2t and 2t+1 of the block */
+    float o[Blocks][S::kPieces][4];
+    float top[Blocks][2], sum[Blocks][2];
+    bool entered = false, at_first = true;
+    int from = 0, stage = 0, first_head = 0, live_heads = 0;
+    for (int done = 0; done < count; ++done) {
+        if (!entered) { /* a new item */
+            entered = true, from = use.tile;
+            first_head = use.kv_head * task.group + use.head_block * 8 * Blocks;
+            live_heads = task.group - use.head_block * 8 * Blocks;
 #pragma unroll
-        for (int s = 0; s < S::kStages - 1; ++s)
-            issue(from + s);
-
-        /* Q^T as the column operand: lane (g, t) holds head g */
-        uint32_t qf[Blocks][Depth / 16][2];
-        float head_scale[Blocks][2]; /* of heads 2t and 2t+1 of the block */
+            for (int n = 0; n < Blocks; ++n) {
+                const bool live = 8 * n + g < live_heads;
+                const __nv_bfloat16 *q = task.q + use.sequence * task.q_batch +
+                                         (live ? first_head + 8 * n + g : 0) * task.q_head;
+                if constexpr (!Eight) {
 #pragma unroll
-        for (int n = 0; n < Blocks; ++n) {
-            const bool live = 8 * n + g < live_heads;
-            const __nv_bfloat16 *q = task.q + sequence * task.q_batch +
-                                     (live ? first_head + 8 * n + g : 0) * task.q_head;
-            if constexpr (!Eight) {
+                    for (int kk = 0; kk < S::kPieces; ++kk)
 #pragma unroll
-                for (int kk = 0; kk < Depth / 16; ++kk)
+                        for (int i = 0; i < 2; ++i) {
+                            const int d = 16 * kk + 8 * i + 2 * t;
+                            qf[n][kk][i] =
+                                live && d < task.depth ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
+                        }
+                    head_scale[n][0] = head_scale[n][1] = task.score_scale;
+                } else {
+                    /* To FP16, whose mantissa holds a BF16 but whose range does not: divided by
+                     * a power of two that brings the head's largest element to [1, 2). */
+                    uint2 raw[S::kPieces];
+                    float largest = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int d = 16 * kk + 8 * i + 2 * t;
-                        qf[n][kk][i] = live && d < task.depth
-                                           ? *reinterpret_cast<const uint32_t *>(q + d)
-                                           : 0u;
+                    for (int kk = 0; kk < S::kPieces; ++kk) {
+                        const int d = 16 * kk + 4 * t;
+                        raw[kk] = live && d < task.depth ? *reinterpret_cast<const uint2 *>(q + d)
+                                                         : make_uint2(0, 0);
+                        const heads::Piece p = heads::unpack_piece(raw[kk]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            largest = fmaxf(largest, fabsf(p.e[i]));
                     }
-                head_scale[n][0] = head_scale[n][1] = task.score_scale;
-            } else {
-                /* To FP16, whose mantissa holds a BF16 but whose range does not: divided by
-                 * a power of two that brings the head's largest element to [1, 2). */
-                uint2 raw[Depth / 16];
-                float largest = 0.f;
+                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                    int exponent = 0; /* of zero and of what is not finite: 0 */
+                    if (largest > 0.f && largest < INFINITY)
+                        exponent = max(-126, min(126, (__float_as_int(largest) >> 23) - 127));
+                    const float down = __int_as_float((127 - exponent) << 23);
+                    const float up = __int_as_float((127 + exponent) << 23);
 #pragma unroll
-                for (int kk = 0; kk < Depth / 16; ++kk) {
-                    const int d = 16 * kk + 4 * t;
-                    raw[kk] = live && d < task.depth ? *reinterpret_cast<const uint2 *>(q + d)
-                                                     : make_uint2(0, 0);
-                    const heads::Piece p = heads::load_piece(
-                        reinterpret_cast<const __nv_bfloat16 *>(&raw[kk]));
+                    for (int kk = 0; kk < S::kPieces; ++kk) {
+                        const heads::Piece p = heads::unpack_piece(raw[kk]);
+                        qf[n][kk][0] = pack<true>(p.e[0] * down, p.e[1] * down);
+                        qf[n][kk][1] = pack<true>(p.e[2] * down, p.e[3] * down);
+                    }
+                    /* lane (g, t) needs the factors of heads 2t and 2t+1, held by lanes 4*(2t + i) */
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        largest = fmaxf(largest, fabsf(p.e[i]));
+                    for (int i = 0; i < 2; ++i)
+                        head_scale[n][i] = task.score_scale * __shfl_sync(0xffffffffu, up, 4 * (2 * t + i));
                 }
-                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                int exponent = 0;
-                if (largest > 0.f && largest < INFINITY)
-                    exponent = ilogbf(largest);
-                exponent = max(-126, min(126, exponent));
-                const float down = exp2f(float(-exponent)), up = exp2f(float(exponent));
 #pragma unroll
-                for (int kk = 0; kk < Depth / 16; ++kk) {
-                    const heads::Piece p = heads::load_piece(
-                        reinterpret_cast<const __nv_bfloat16 *>(&raw[kk]));
-                    qf[n][kk][0] = pack<true>(p.e[0] * down, p.e[1] * down);
-                    qf[n][kk][1] = pack<true>(p.e[2] * down, p.e[3] * down);
-                }
-                /* lane (g, t) needs the factors of heads 2t and 2t+1, held by lanes 4*(2t + i) */
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    head_scale[n][i] =
-                        task.score_scale * __shfl_sync(0xffffffffu, up, 4 * (2 * t + i));
+                for (int j = 0; j < S::kPieces; ++j)
+                    o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+                top[n][0] = top[n][1] = -INFINITY;
+                sum[n][0] = sum[n][1] = 0.f;
             }
         }
 
-        float o[Blocks][Depth / 16][4];
-        float top[Blocks][2], sum[Blocks][2];
+        copy(stage == 0 ? S::kStages - 1 : stage - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+        __syncwarp();
+        const uint32_t keys = ring + stage * S::kTileBytes;
+        const uint32_t values = keys + S::kTile * S::kRowBytes;
+        uint32_t real[kOwn], any = 0;
 #pragma unroll
-        for (int n = 0; n < Blocks; ++n) {
-#pragma unroll
-            for (int j = 0; j < Depth / 16; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    o[n][j][i] = 0.f;
-            top[n][0] = top[n][1] = -INFINITY;
-            sum[n][0] = sum[n][1] = 0.f;
+        for (int i = 0; i < kOwn; ++i) {
+            real[i] = reinterpret_cast<const uint32_t *>(notes + stage * S::kNoteBytes + 16 * S::kTile)[i];
+            any |= real[i];
         }
-
-        for (int j = from; j < upto; ++j) {
-            issue(j + S::kStages - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
-            __syncwarp();
-            const int stage = (j - from) % S::kStages;
-            const uint32_t keys = ring + stage * S::kStageBytes;
-            const uint32_t values = keys + kWarpTokens * S::kRowBytes;
-            const uint32_t real = seen_words[stage];
-            if (real) {
-                float s[Blocks][4];
+        if (any) {
+            /* scores of tokens 16m + g and 16m + g + 8; a single group has two chains of products,
+             * added afterwards */
+            constexpr int kChains = S::kGroups == 1 ? 2 : 1;
+            float s[Blocks][S::kGroups][kChains][4];
 #pragma unroll
-                for (int n = 0; n < Blocks; ++n)
-                    s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            for (int n = 0; n < Blocks; ++n)
 #pragma unroll
-                for (int kk = 0; kk < Depth / 16; ++kk) {
+                for (int m = 0; m < S::kGroups; ++m)
+#pragma unroll
+                    for (int c = 0; c < kChains; ++c)
+                        s[n][m][c][0] = s[n][m][c][1] = s[n][m][c][2] = s[n][m][c][3] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < S::kPieces; ++kk)
+#pragma unroll
+                for (int m = 0; m < S::kGroups; ++m) {
                     uint32_t a[4];
                     if constexpr (!Eight) {
-                        const int row = lane & 15, chunk = 2 * kk + lane / 16;
-                        ldmatrix_x4(a, keys + row * S::kRowBytes + S::place(row, chunk));
+                        const int row = 16 * m + (lane & 15), part = 2 * kk + lane / 16;
+                        ldmatrix_x4(a, keys + row * S::kRowBytes + S::place(row, part));
                     } else {
                         /* lane (g, t) takes depths 16 kk + 4t .. + 3 of tokens g and g + 8; the
                          * query operand is in the same order */
-                        const uint32_t at = S::place(g, kk) + 4 * t;
+                        const uint32_t at = keys + (16 * m + g) * S::kRowBytes + S::place(g, kk) + 4 * t;
                         uint32_t low, high;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(low) : "r"(keys + g * S::kRowBytes + at));
-                        asm volatile("ld.shared.u32 %0, [%1];"
-                                     : "=r"(high)
-                                     : "r"(keys + (g + 8) * S::kRowBytes + at));
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(low) : "r"(at));
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(high) : "r"(at + 8 * S::kRowBytes));
                         a[0] = widen(low & 0xffff), a[1] = widen(high & 0xffff);
                         a[2] = widen(low >> 16), a[3] = widen(high >> 16);
                     }
 #pragma unroll
                     for (int n = 0; n < Blocks; ++n)
-                        mma_16816<Eight>(s[n], a, qf[n][kk][0], qf[n][kk][1]);
+                        mma_16816<Eight>(s[n][m][kk % kChains], a, qf[n][kk][0], qf[n][kk][1]);
                 }
-                const bool low_real = (real >> g) & 1, high_real = (real >> (g + 8)) & 1;
-                uint32_t p[Blocks][2];
-                bool rescale = false;
-                float factor[Blocks][2];
+            uint32_t p[Blocks][S::kGroups][2];
+            bool rescale = false;
+            float factor[Blocks][2];
 #pragma unroll
-                for (int n = 0; n < Blocks; ++n) {
-                    float weight[4];
+            for (int n = 0; n < Blocks; ++n) {
+                float score[S::kGroups][4], best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float a = low_real ? s[n][i] * head_scale[n][i] : -INFINITY;
-                        const float b = high_real ? s[n][i + 2] * head_scale[n][i] : -INFINITY;
-                        float best = fmaxf(a, b);
+                for (int m = 0; m < S::kGroups; ++m)
 #pragma unroll
-                        for (int offset = 4; offset < 32; offset *= 2)
-                            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, offset));
-                        best = fmaxf(best, top[n][i]);
-                        const float reference = best == -INFINITY ? 0.f : best;
-                        factor[n][i] = exp2f(top[n][i] - reference);
-                        rescale = rescale || best != top[n][i];
-                        top[n][i] = best;
-                        weight[i] = exp2f(a - reference), weight[i + 2] = exp2f(b - reference);
-                        sum[n][i] = sum[n][i] * factor[n][i] + weight[i] + weight[i + 2];
+                    for (int i = 0; i < 4; ++i) {
+                        float value = s[n][m][0][i];
+                        if constexpr (kChains == 2)
+                            value += s[n][m][1][i];
+                        const bool seen = (real[m / 2] >> (16 * (m % 2) + g + 8 * (i / 2))) & 1;
+                        score[m][i] = seen ? value * head_scale[n][i & 1] : -INFINITY;
+                        best[i & 1] = fmaxf(best[i & 1], score[m][i]);
                     }
-                    p[n][0] = transpose_8x8(pack<Eight>(weight[0], weight[1]));
-                    p[n][1] = transpose_8x8(pack<Eight>(weight[2], weight[3]));
+                float reference[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int offset = 4; offset < 32; offset *= 2)
+                        best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], offset));
+                    best[i] = fmaxf(best[i], top[n][i]);
+                    reference[i] = best[i] == -INFINITY ? 0.f : best[i];
+                    factor[n][i] = power_of_two(top[n][i] - reference[i]);
+                    rescale = rescale || best[i] != top[n][i];
+                    top[n][i] = best[i];
+                    sum[n][i] *= factor[n][i];
                 }
-                if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-                    for (int n = 0; n < Blocks; ++n)
+                for (int m = 0; m < S::kGroups; ++m) {
 #pragma unroll
-                        for (int jj = 0; jj < Depth / 16; ++jj)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                o[n][jj][i] *= factor[n][i & 1];
+                    for (int i = 0; i < 4; ++i) {
+                        score[m][i] = power_of_two(score[m][i] - reference[i & 1]);
+                        sum[n][i & 1] += score[m][i];
+                    }
+                    p[n][m][0] = transpose_8x8(pack<Eight>(score[m][0], score[m][1]));
+                    p[n][m][1] = transpose_8x8(pack<Eight>(score[m][2], score[m][3]));
                 }
+            }
+            if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+                for (int n = 0; n < Blocks; ++n)
+#pragma unroll
+                    for (int j = 0; j < S::kPieces; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            o[n][j][i] *= factor[n][i & 1];
+            }
+#pragma unroll
+            for (int m = 0; m < S::kGroups; ++m) {
                 if constexpr (!Eight) {
 #pragma unroll
-                    for (int jj = 0; jj < Depth / 16; ++jj) {
+                    for (int j = 0; j < S::kPieces; ++j) {
                         uint32_t a[4];
-                        const int row = (lane & 7) + (lane / 16) * 8, chunk = 2 * jj + ((lane / 8) & 1);
-                        ldmatrix_x4_trans(a, values + row * S::kRowBytes + S::place(row, chunk));
+                        const int row = 16 * m + (lane & 7) + (lane / 16) * 8, part = 2 * j + ((lane / 8) & 1);
+                        ldmatrix_x4_trans(a, values + row * S::kRowBytes + S::place(row, part));
 #pragma unroll
                         for (int n = 0; n < Blocks; ++n)
-                            mma_16816<false>(o[n][jj], a, p[n][0], p[n][1]);
+                            mma_16816<false>(o[n][j], a, p[n][m][0], p[n][m][1]);
                     }
                 } else {
                     /* lane (g, t): depths 32 J + 4g + i, i = 0..3, of tokens 2t, 2t+1, 2t+8, 2t+9:
                      * row g of product 2J is depth 32 J + 4g, row g + 8 the next one, and so on */
 #pragma unroll
-                    for (int J = 0; J < Depth / 32; ++J) {
+                    for (int J = 0; J < S::kPieces / 2; ++J) {
                         uint32_t word[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int row = 2 * t + (i & 1) + (i / 2) * 8;
-                            const uint32_t at = values + row * S::kRowBytes +
-                                                S::place(row, 2 * J + g / 4) + 4 * (g % 4);
+                            const int row = 16 * m + 2 * t + (i & 1) + (i / 2) * 8;
+                            const uint32_t at =
+                                values + row * S::kRowBytes + S::place(row, 2 * J + g / 4) + 4 * (g % 4);
                             asm volatile("ld.shared.u32 %0, [%1];" : "=r"(word[i]) : "r"(at));
                         }
                         const uint32_t low01 = __byte_perm(word[0], word[1], 0x5140);
                         const uint32_t high01 = __byte_perm(word[0], word[1], 0x7362);
                         const uint32_t low23 = __byte_perm(word[2], word[3], 0x5140);
                         const uint32_t high23 = __byte_perm(word[2], word[3], 0x7362);
-                        const uint32_t even[4] = {widen(low01 & 0xffff), widen(low01 >> 16),
-                                                  widen(low23 & 0xffff), widen(low23 >> 16)};
-                        const uint32_t odd[4] = {widen(high01 & 0xffff), widen(high01 >> 16),
-                                                 widen(high23 & 0xffff), widen(high23 >> 16)};
+                        const uint32_t even[4] = {widen(low01 & 0xffff), widen(low01 >> 16), widen(low23 & 0xffff),
+                                                  widen(low23 >> 16)};
+                        const uint32_t odd[4] = {widen(high01 & 0xffff), widen(high01 >> 16), widen(high23 & 0xffff),
+                                                 widen(high23 >> 16)};
 #pragma unroll
                         for (int n = 0; n < Blocks; ++n) {
-                            mma_16816<true>(o[n][2 * J], even, p[n][0], p[n][1]);
-                            mma_16816<true>(o[n][2 * J + 1], odd, p[n][0], p[n][1]);
+                            mma_16816<true>(o[n][2 * J], even, p[n][m][0], p[n][m][1]);
+                            mma_16816<true>(o[n][2 * J + 1], odd, p[n][m][0], p[n][m][1]);
                         }
                     }
                 }
             }
-            __syncwarp();
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp(); /* all lanes are done with the stage that the next copy fills */
+        stage = stage + 1 == S::kStages ? 0 : stage + 1;
 
-        /* join the four warps, then write the result or this CTA's piece of it */
+        const bool item_ends = use.tile + 1 == use.view.tiles;
+        if (item_ends || done + 1 == count) {
+            const bool whole = item_ends && from == 0;
+            const long long piece = 2ll * global_warp + (at_first ? 0 : 1);
 #pragma unroll
-        for (int n = 0; n < Blocks; ++n)
+            for (int n = 0; n < Blocks; ++n) {
+                float inverse[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int offset = 4; offset < 32; offset *= 2)
-                    sum[n][i] += __shfl_xor_sync(0xffffffffu, sum[n][i], offset);
-                const int head = 8 * n + 2 * t + i;
-                if (g == 0) {
-                    join_stats[(warp * S::kHeads + head) * 2] = top[n][i];
-                    join_stats[(warp * S::kHeads + head) * 2 + 1] = sum[n][i];
+                    for (int offset = 4; offset < 32; offset *= 2)
+                        sum[n][i] += __shfl_xor_sync(0xffffffffu, sum[n][i], offset);
+                    inverse[i] = sum[n][i] != 0.f ? task.value_scale / sum[n][i] : 0.f;
+                    if (!whole && g == 0)
+                        task.statistics[(piece * Blocks + n) * 8 + 2 * t + i] = make_float2(top[n][i], sum[n][i]);
                 }
-                float *to = join + (warp * S::kHeads + head) * S::kJoinPitch;
+                __nv_bfloat16 *out =
+                    task.out + ((long long)use.sequence * task.heads + first_head + 8 * n) * task.depth;
 #pragma unroll
-                for (int jj = 0; jj < Depth / 16; ++jj) {
-                    /* rows g and g + 8 of product jj */
-                    const int d = Eight ? 32 * (jj / 2) + 4 * g + 2 * (jj & 1) : 16 * jj + g;
-                    to[d] = o[n][jj][i];
-                    to[d + (Eight ? 1 : 8)] = o[n][jj][i + 2];
-                }
-            }
-        __syncthreads();
-        const bool whole = from == 0 && upto == tiles;
-        const long long piece = 2ll * blockIdx.x + (tile == begin ? 0 : 1);
-        for (int at = threadIdx.x; at < live_heads * task.depth; at += kWarps * 32) {
-            const int head = at / task.depth, d = at - head * task.depth;
-            float best = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w)
-                best = fmaxf(best, join_stats[(w * S::kHeads + head) * 2]);
-            const float reference = best == -INFINITY ? 0.f : best;
-            float value = 0.f, weight = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float factor = exp2f(join_stats[(w * S::kHeads + head) * 2] - reference);
-                weight += factor * join_stats[(w * S::kHeads + head) * 2 + 1];
-                value += factor * join[(w * S::kHeads + head) * S::kJoinPitch + d];
-            }
-            if (whole) {
-                const long long row = (long long)sequence * task.heads + first_head + head;
-                task.out[row * task.depth + d] = __float2bfloat16_rn(
-                    weight != 0.f ? value * task.value_scale / weight : 0.f);
-            } else {
-                task.pieces[(piece * S::kHeads + head) * task.depth + d] = value;
-                if (d == 0) {
-                    task.statistics[(piece * S::kHeads + head) * 2] = best;
-                    task.statistics[(piece * S::kHeads + head) * 2 + 1] = weight;
+                for (int j = 0; j < S::kPieces; ++j) {
+                    if (whole)
+                        store_heads<Eight>(out, task.depth, live_heads - 8 * n, j, o[n][j], inverse);
+                    else
+                        task.pieces[((piece * Blocks + n) * S::kPieces + j) * 32 + lane] =
+                            make_float4(o[n][j][0], o[n][j][1], o[n][j][2], o[n][j][3]);
                 }
             }
+            entered = false, at_first = false;
         }
-        __syncthreads();
-        tile = item_first + upto;
-        if (tile >= sequence_first + (long long)tiles * task.kv_heads * task.head_blocks) {
-            sequence_first += (long long)tiles * task.kv_heads * task.head_blocks;
-            ++sequence;
-        }
+        use.advance(task, member);
     }
 }
 
-/* Adds the pieces of every item that more than one CTA worked on, in token
- * order. One CTA per item; `grid` and `slots` (heads per piece) are those of the
- * attend kernel, whose programmatic dependent this kernel is. */
-__global__ void __launch_bounds__(128) attend_join(const AttendTask task, int grid, int slots)
+/* Adds the pieces of an item that more than one worker took part in, in token
+ * order; a programmatic dependent of attend_kernel. blockIdx.x: item and column
+ * block, blockIdx.y: 32 * kJoinProducts depths. The warps of a CTA each take a
+ * contiguous share of the pieces, kJoinAtOnce in flight; their sums are added
+ * through shared memory. */
+constexpr int kJoinWarps = 16; /* at most */
+constexpr int kJoinProducts = 2;
+constexpr int kJoinAtOnce = 4;
+
+template <bool Eight>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    attend_join(const __grid_constant__ AttendTask task, int blocks, int depth_pieces)
 {
-    const int per = task.kv_heads * task.head_blocks;
-    const int sequence = blockIdx.x / per, item = blockIdx.x % per;
-    const long long total = total_tiles(task);
-    long long before = 0;
-    for (int b = threadIdx.x & 31; b < sequence; b += 32)
-        before += tiles_of(task, b);
-#pragma unroll
-    for (int offset = 16; offset > 0; offset /= 2)
-        before += __shfl_xor_sync(0xffffffffu, before, offset);
-    const int tiles = tiles_of(task, sequence);
-    const long long first = before * per + (long long)item * tiles, last = first + tiles - 1;
-    /* the CTA of a tile: the last one whose range starts at or before it */
-    const auto owner = [&](long long tile) {
-        int low = 0, high = grid - 1;
-        while (low < high) {
-            const int middle = (low + high + 1) / 2;
-            if (range_start(total, grid, middle) <= tile)
-                low = middle;
-            else
-                high = middle - 1;
-        }
-        return low;
-    };
-    const int from = owner(first), upto = owner(last);
+    __shared__ float4 shared_sum[kJoinWarps][kJoinProducts][32];
+    __shared__ float shared_stats[kJoinWarps][2][8];
+    const int part = threadIdx.x / 32, parts = blockDim.x / 32;
+    const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const int n = blockIdx.x % blocks, item = blockIdx.x / blocks;
+    const int product = blockIdx.y * kJoinProducts;
+    const int slots = task.team * task.teams;
+    const int sequence = item / slots, slot = item % slots;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const long long sequence_first = __ldcg(&task.first_tile[sequence]);
+    const int tiles = int((__ldcg(&task.first_tile[sequence + 1]) - sequence_first) / task.teams);
+    const long long first = sequence_first + (long long)(slot / task.team) * tiles;
+    const Cut cut(__ldcg(&task.first_tile[task.batch]), task.workers);
+    const int from = cut.owner(first), upto = cut.owner(first + tiles - 1);
     if (from == upto)
         return; /* written whole */
-    const int kv_head = item / task.head_blocks, head_block = item % task.head_blocks;
-    const int first_head = kv_head * task.group + head_block * slots;
-    const int live_heads = min(slots, task.group - head_block * slots);
-    const int first_slot = range_start(total, grid, from) < first ? 1 : 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int at = threadIdx.x; at < live_heads * task.depth; at += blockDim.x) {
-        const int head = at / task.depth, d = at - head * task.depth;
-        float best = -INFINITY, weight = 0.f, value = 0.f;
-        for (int cta = from; cta <= upto; ++cta) {
-            if (cta != from && cta != upto && range_start(total, grid, cta) == range_start(total, grid, cta + 1))
-                continue;
-            const long long piece = (2ll * cta + (cta == from ? first_slot : 0)) * slots + head;
-            const float top = task.statistics[piece * 2], part = task.statistics[piece * 2 + 1];
-            const float higher = fmaxf(best, top);
-            const float reference = higher == -INFINITY ? 0.f : higher;
-            const float old = exp2f(best - reference), fresh = exp2f(top - reference);
-            weight = weight * old + part * fresh;
-            value = value * old + task.pieces[piece * task.depth + d] * fresh;
-            best = higher;
+    const int member = slot % task.team;
+    const int first_place = cut.start(from) < first ? 1 : 0;
+    const int share = (upto - from + parts) / parts;
+    const int begin = from + part * share, end = min(upto + 1, begin + share);
+    float sum[kJoinProducts][4] = {};
+    float top[2] = {-INFINITY, -INFINITY}, weight[2] = {0.f, 0.f};
+    for (int base = begin; base < end; base += kJoinAtOnce) {
+        float4 value[kJoinAtOnce][kJoinProducts];
+        float2 stats[kJoinAtOnce][2];
+#pragma unroll
+        for (int i = 0; i < kJoinAtOnce; ++i) {
+            const int worker = min(base + i, end - 1);
+            const long long piece =
+                (2ll * (worker * task.team + member) + (worker == from ? first_place : 0)) * blocks + n;
+#pragma unroll
+            for (int c = 0; c < kJoinProducts; ++c)
+                value[i][c] = __ldcg(&task.pieces[(piece * depth_pieces + product + c) * 32 + lane]);
+            stats[i][0] = __ldcg(&task.statistics[piece * 8 + 2 * t]);
+            stats[i][1] = __ldcg(&task.statistics[piece * 8 + 2 * t + 1]);
         }
-        const long long row = (long long)sequence * task.heads + first_head + head;
-        task.out[row * task.depth + d] =
-            __float2bfloat16_rn(weight != 0.f ? value * task.value_scale / weight : 0.f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float best = top[h];
+#pragma unroll
+            for (int i = 0; i < kJoinAtOnce; ++i)
+                best = fmaxf(best, stats[i][h].x);
+            const float reference = best == -INFINITY ? 0.f : best;
+            const float factor = power_of_two(top[h] - reference);
+            top[h] = best, weight[h] *= factor;
+#pragma unroll
+            for (int c = 0; c < kJoinProducts; ++c)
+                sum[c][h] *= factor, sum[c][h + 2] *= factor;
+#pragma unroll
+            for (int i = 0; i < kJoinAtOnce; ++i) {
+                if (base + i >= end)
+                    break;
+                const float share_of = power_of_two(stats[i][h].x - reference);
+                weight[h] += share_of * stats[i][h].y;
+#pragma unroll
+                for (int c = 0; c < kJoinProducts; ++c) {
+                    sum[c][h] += share_of * (h == 0 ? value[i][c].x : value[i][c].y);
+                    sum[c][h + 2] += share_of * (h == 0 ? value[i][c].z : value[i][c].w);
+                }
+            }
+        }
     }
+#pragma unroll
+    for (int c = 0; c < kJoinProducts; ++c)
+        shared_sum[part][c][lane] = make_float4(sum[c][0], sum[c][1], sum[c][2], sum[c][3]);
+    if (g == 0)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            shared_stats[part][0][2 * t + h] = top[h], shared_stats[part][1][2 * t + h] = weight[h];
+    __syncthreads();
+    if (part >= kJoinProducts)
+        return;
+    /* warp c finishes product c */
+    float total[2] = {0.f, 0.f}, result[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float best = -INFINITY;
+        for (int other = 0; other < parts; ++other)
+            best = fmaxf(best, shared_stats[other][0][2 * t + h]);
+        const float reference = best == -INFINITY ? 0.f : best;
+        for (int other = 0; other < parts; ++other) {
+            const float factor = power_of_two(shared_stats[other][0][2 * t + h] - reference);
+            const float4 v = shared_sum[other][part][lane];
+            total[h] += factor * shared_stats[other][1][2 * t + h];
+            result[h] += factor * (h == 0 ? v.x : v.y);
+            result[h + 2] += factor * (h == 0 ? v.z : v.w);
+        }
+        total[h] = total[h] != 0.f ? task.value_scale / total[h] : 0.f;
+    }
+    const int head_block = slot % task.head_blocks;
+    const int first_head = slot / task.head_blocks * task.group + (head_block * blocks + n) * 8;
+    const int live_heads = task.group - (head_block * blocks + n) * 8;
+    store_heads<Eight>(task.out + ((long long)sequence * task.heads + first_head) * task.depth, task.depth,
+                       live_heads, product + part, result, total);
 }
 
 /* How one call is cut: kernel instance, CTAs, workspace. */
 struct Plan {
     int depth_class = 0; /* 64, 128 or 256 */
-    int blocks = 1;
-    int head_blocks = 1;
+    int blocks = 1, head_blocks = 1, team = 1, teams = 1;
     long long tiles_bound = 0; /* most tiles an item can have */
-    int grid = 0;
-    size_t bytes = 0;
+    int grid = 0, workers = 0, tile_shift = 0;
+    size_t first_bytes = 0, piece_bytes = 0, bytes = 0;
 };
 
 /* Calls work(Shape<...>) for the instance that a call uses. */
@@ -660,16 +841,28 @@ inline Plan make_plan(int sm_count, int batch, int heads_count, int kv_heads, in
      * does not fit the registers at 256 columns; there the second block of heads reads again. */
     plan.blocks = group > 8 && plan.depth_class <= 128 ? 2 : 1;
     plan.head_blocks = (group + 8 * plan.blocks - 1) / (8 * plan.blocks);
+    const int slots = kv_heads * plan.head_blocks;
+    plan.team = slots % 4 == 0 ? 4 : (slots % 2 == 0 ? 2 : 1);
+    plan.teams = slots / plan.team;
     long long bound = (long long)page_size * table_width;
     if (window > 0 && bound > (long long)window + sinks)
         bound = (long long)window + sinks;
-    plan.tiles_bound = bound > kTile ? (bound + kTile - 1) / kTile : 1;
-    const int resident = with_shape(plan.depth_class, plan.blocks, cache_type == 3,
-                                    [](auto shape) { return decltype(shape)::kResident; });
-    const long long most = plan.tiles_bound * batch * kv_heads * plan.head_blocks;
+    bound = bound < INT_MAX ? bound : INT_MAX;
+    const bool eight = cache_type == 3;
+    plan.tile_shift =
+        with_shape(plan.depth_class, plan.blocks, eight, [](auto shape) { return decltype(shape)::kTileShift; });
+    plan.tiles_bound = bound > 0 ? ((bound - 1) >> plan.tile_shift) + 1 : 1;
+    const int resident =
+        with_shape(plan.depth_class, plan.blocks, eight, [](auto shape) { return decltype(shape)::kResident; });
+    const long long warps = plan.tiles_bound * batch * slots;
+    const long long most = (warps + kWarps - 1) / kWarps;
     const long long full = (long long)sm_count * resident;
     plan.grid = int(most < full ? most : full);
-    plan.bytes = size_t(plan.grid) * 2 * 8 * plan.blocks * (size_t(depth) + 2) * 4;
+    plan.workers = plan.grid * kWarps / plan.team;
+    plan.first_bytes = (size_t(batch) + 1 + 1) / 2 * 16;
+    const size_t held = plan.tiles_bound > 1 ? size_t(plan.grid) * kWarps * 2 * plan.blocks : 0;
+    plan.piece_bytes = held * (plan.depth_class / 16) * 32 * 16;
+    plan.bytes = plan.first_bytes + plan.piece_bytes + held * 8 * 8;
     return plan;
 }
 
@@ -678,6 +871,27 @@ void launch(camblas_cuda_context *context, const AttendTask &task, const Plan &p
 {
     attend_kernel<Depth, Blocks, Eight>
         <<<plan.grid, kWarps * 32, Shape<Depth, Blocks, Eight>::kBytes, context->stream>>>(task);
+}
+
+template <bool Eight>
+cudaError_t launch_join(camblas_cuda_context *context, const AttendTask &task, const Plan &plan)
+{
+    /* Pieces per item if the lengths are alike; ragged ones give long items many more, so at
+     * least four warps share an item's pieces unless there are items for every warp of the chip. */
+    const int items = task.batch * plan.team * plan.teams;
+    const int expected = plan.grid * kWarps / items + 2;
+    const int parts = expected >= 64 ? 16 : (expected >= 32 ? 8 : (expected > 4 ? 4 : 2));
+    const int depth_pieces = plan.depth_class / 16;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(items) * plan.blocks, depth_pieces / kJoinProducts);
+    config.blockDim = dim3(parts * 32);
+    config.stream = context->stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, attend_join<Eight>, task, plan.blocks, depth_pieces);
 }
 
 template <int Depth, int Blocks, bool Eight> int allow_shared(Shape<Depth, Blocks, Eight>)
@@ -756,9 +970,13 @@ extern "C" int camblas_cuda_paged_attention(
                                                     cache_type, page_size, table_width, window, sinks);
         if (workspace_bytes < plan.bytes || !workspace || heads::misaligned(workspace, 16))
             return host::fail(context, "paged attention workspace too small", 1);
-        task.batch = batch, task.heads = heads_count, task.kv_heads = kv_heads;
-        task.group = heads_count / kv_heads, task.head_blocks = plan.head_blocks, task.depth = depth;
-        task.page_size = page_size, task.pages = pages, task.table_width = table_width;
+        task.batch = batch, task.heads = heads_count, task.group = heads_count / kv_heads, task.depth = depth;
+        task.head_blocks = plan.head_blocks, task.team = plan.team, task.teams = plan.teams;
+        task.workers = plan.workers;
+        for (heads::CacheLayout *cache : {&task.keys, &task.values})
+            cache->page_stride *= element, cache->slot_stride *= element, cache->head_stride *= element;
+        task.page_size = page_size, task.pages = pages, task.tile_shift = plan.tile_shift;
+        task.room = int(std::min<long long>((long long)table_width * page_size, INT_MAX));
         task.page_shift = -1;
         for (int shift = 0; shift < 31; ++shift)
             if (page_size == 1 << shift)
@@ -771,8 +989,10 @@ extern "C" int camblas_cuda_paged_attention(
         task.score_scale = scale * key_scale * 1.4426950408889634f;
         task.value_scale = value_scale;
         task.out = static_cast<__nv_bfloat16 *>(output);
-        task.pieces = static_cast<float *>(workspace);
-        task.statistics = task.pieces + size_t(plan.grid) * 2 * 8 * plan.blocks * depth;
+        char *held = static_cast<char *>(workspace);
+        task.first_tile = reinterpret_cast<long long *>(held);
+        task.pieces = reinterpret_cast<float4 *>(held + plan.first_bytes);
+        task.statistics = reinterpret_cast<float2 *>(held + plan.first_bytes + plan.piece_bytes);
         context->counts[6]++;
         attend::with_shape(plan.depth_class, plan.blocks, cache_type == 3, [&](auto shape) {
             attend::launch(context, task, plan, shape);
@@ -781,16 +1001,8 @@ extern "C" int camblas_cuda_paged_attention(
         const int status = host::launched(context, "paged attention");
         if (status != 0 || plan.tiles_bound == 1)
             return status;
-        cudaLaunchConfig_t config = {};
-        config.gridDim = dim3(unsigned(batch) * kv_heads * plan.head_blocks);
-        config.blockDim = dim3(128);
-        config.stream = context->stream;
-        cudaLaunchAttribute attribute[1];
-        attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attribute[0].val.programmaticStreamSerializationAllowed = 1;
-        config.attrs = attribute;
-        config.numAttrs = 1;
-        const cudaError_t error = cudaLaunchKernelEx(&config, attend::attend_join, task, plan.grid, 8 * plan.blocks);
+        const cudaError_t error = cache_type == 3 ? attend::launch_join<true>(context, task, plan)
+                                                  : attend::launch_join<false>(context, task, plan);
         if (error != cudaSuccess)
             return host::fail(context, "paged attention join", error);
         context->kernel_launches.fetch_add(1, std::memory_order_relaxed);

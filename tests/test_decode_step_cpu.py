@@ -64,9 +64,13 @@ def test_rotary_table_is_formed_in_64_bits():
 @pytest.mark.parametrize("tiles,per,grid", [((1,), 1, 1), ((1, 1, 1), 8, 296), ((40, 1, 7), 3, 16),
                                             ((2047,), 8, 296), ((1, 300, 2, 5), 2, 148)])
 def test_equal_ranges_cover_every_tile_once(tiles, per, grid):
-    """The cut of the paged attention: ranges, their pieces' places, and the CTAs an item finds its pieces at."""
+    """The cut of the paged attention: ranges, their pieces' places, and the workers an item finds its pieces at."""
     def start(cta):
-        return total // grid * cta + total % grid * cta // grid
+        return total // grid * cta + min(cta, total % grid)
+
+    def owner(tile):
+        each, longer = divmod(total, grid)
+        return tile // (each + 1) if tile < longer * (each + 1) else longer + (tile - longer * (each + 1)) // each
 
     total = sum(tiles) * per
     written, pieces = {}, {}
@@ -95,6 +99,7 @@ def test_equal_ranges_cover_every_tile_once(tiles, per, grid):
         for item in range(per):
             first = sum(tiles[:sequence]) * per + item * count
             owners = sorted({written[sequence, item, j] for j in range(count)})
+            assert owners == list(range(owner(first), owner(first + count - 1) + 1))
             if len(owners) == 1:
                 continue
             reached = 0
