@@ -756,7 +756,7 @@ def _heads_operand(tensor, index):
     _require(index >= 0 and tensor.get_device() == index and tensor.dtype is torch.bfloat16
              and tensor.dim() == 3, "Heads must be CUDA BF16 [rows, heads, depth] on one device")
     row, head, unit = tensor.stride()
-    if unit != 1 or row % 4 or head % 4 or tensor.data_ptr() % 8:
+    if unit != 1 or row % 4 or head % 4 or head > _INT_MAX or tensor.data_ptr() % 8:
         tensor = tensor.clone(memory_format=torch.contiguous_format)
         row, head, unit = tensor.stride()
     return tensor, row, head

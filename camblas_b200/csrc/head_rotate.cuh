@@ -12,9 +12,8 @@
  * cache, from FP32 straight to E4M3.
  *
  * The reads and writes of the heads bound the kernel: seven operations per
- * element against four bytes. The
- * largest power of two of lanes that a depth needs (eight elements per lane)
- * shares a head; a lane holds both members of its pairs, so the rotation needs
+ * element against four bytes. As many lanes as a depth needs at eight elements
+ * per lane, rounded up to a power of two, share a head; a lane holds both members of its pairs, so the rotation needs
  * no exchange and the norm one shuffle tree. A lane's eight elements are two
  * 8-byte pieces, which for the half-split form lie rotary/2 apart.
  */
@@ -30,7 +29,10 @@
 namespace heads
 {
 
-constexpr int kThreads = 256;
+/* Two warps: with 64 + 8 heads of 128 a lane turns 16 query heads and 2 key heads, over which its
+ * preparation is spread (8192 tokens: 85 us with 256 threads, 68 with 128, 62 with 64). */
+constexpr int kThreads = 64;
+constexpr int kBatch = 4; /* heads of a lane that are fetched together */
 
 /* Address of head h of one cached token: base + page*page_stride +
  * slot*slot_stride + h*head_stride, in elements. */
@@ -42,9 +44,10 @@ struct CacheLayout {
 struct RotateTask {
     int tokens, heads, kv_heads, depth, rotary, table_rows, page_size;
     int interleaved, eight_bit;
-    float epsilon, key_scale, value_scale;
+    float epsilon, inverse_depth, key_scale, value_scale;
     const __nv_bfloat16 *q, *k, *v; /* v NULL: no cache */
-    long long q_token, q_head, k_token, k_head, v_token, v_head;
+    long long q_token, k_token, v_token; /* strides */
+    int q_head, k_head, v_head;
     const __nv_bfloat16 *q_weight, *k_weight;
     const int64_t *positions, *slots;
     const float *table;
@@ -89,120 +92,265 @@ __device__ __forceinline__ void store_piece_e4m3(uint8_t *to, const Piece &p, fl
     *reinterpret_cast<uint32_t *>(to) = low | (high << 16);
 }
 
-/* `Lanes` lanes share a head. Work item = one head of one token, query heads
- * first, then key heads, then (with a cache) value heads. */
-template <int Lanes>
-__global__ void __launch_bounds__(kThreads) rotate_kernel(const RotateTask task)
+/* Two FP32 numbers in a register pair, and the packed arithmetic on them. */
+typedef unsigned long long Two;
+
+__device__ __forceinline__ Two two(float low, float high)
 {
-    const int per_token = task.heads + (task.v ? 2 : 1) * task.kv_heads;
-    const long long items = (long long)task.tokens * per_token;
-    const int unit = threadIdx.x % Lanes;
-    const int turned = task.rotary / 8; /* units that rotate */
-    /* the two 4-element pieces of this lane */
-    const bool split_pair = !task.interleaved && unit < turned;
-    const int first = split_pair ? 4 * unit : 8 * unit;
-    const int second = split_pair ? first + task.rotary / 2 : first + 4;
-    const bool live_unit = 8 * unit < task.depth;
-    constexpr int kPerBlock = kThreads / Lanes;
-    for (long long start = (long long)blockIdx.x * kPerBlock; start < items;
-         start += (long long)gridDim.x * kPerBlock) {
-        const long long item = start + threadIdx.x / Lanes;
-        const bool live = item < items && live_unit;
-        const int token = live ? int(item / per_token) : 0;
-        int head = live ? int(item - (long long)token * per_token) : 0;
-        const __nv_bfloat16 *source, *weight;
-        int kind = 0;
-        if (head < task.heads) {
-            source = task.q + token * task.q_token + head * task.q_head;
-            weight = task.q_weight;
-        } else if (head < task.heads + task.kv_heads) {
-            kind = 1, head -= task.heads;
-            source = task.k + token * task.k_token + head * task.k_head;
-            weight = task.k_weight;
-        } else {
-            kind = 2, head -= task.heads + task.kv_heads;
-            source = task.v + token * task.v_token + head * task.v_head;
-            weight = nullptr;
-        }
-        Piece a{}, b{};
-        long long position = 0, slot = -1;
-        if (live) {
-            a = load_piece(source + first), b = load_piece(source + second);
-            position = task.positions[token];
-            if (kind != 0 && task.v)
-                slot = task.slots[token];
-        }
-        const bool placed = position >= 0 && position < task.table_rows;
-        float square = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            square += a.e[i] * a.e[i] + b.e[i] * b.e[i];
-#pragma unroll
-        for (int offset = Lanes / 2; offset > 0; offset /= 2)
-            square += __shfl_xor_sync(0xffffffffu, square, offset, Lanes);
-        if (!live)
-            continue;
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(low), "f"(high));
+    return r;
+}
+
+__device__ __forceinline__ float2 both(Two x)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+
+__device__ __forceinline__ Two multiply(Two x, Two y)
+{
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+__device__ __forceinline__ Two multiply_add(Two x, Two y, Two z)
+{
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+
+__device__ __forceinline__ Two swapped(Two x)
+{
+    const float2 v = both(x);
+    return two(v.y, v.x);
+}
+
+/* a BF16 pair as FP32 */
+__device__ __forceinline__ Two widen_pair(uint32_t raw)
+{
+    return two(__uint_as_float(raw << 16), __uint_as_float(raw & 0xffff0000u));
+}
+
+/* A lane's eight elements of one head: pieces a and b of four. */
+struct Eight {
+    Two a[2], b[2];
+};
+
+__device__ __forceinline__ Piece as_piece(const Two (&x)[2])
+{
+    const float2 low = both(x[0]), high = both(x[1]);
+    return {{low.x, low.y, high.x, high.y}};
+}
+
+/* What a lane multiplies its elements by: a' = a * straight.a + (b, or a with its
+ * pairs swapped) * cross.a, and b' likewise; the products of the norm's weight
+ * (NULL: 1) and the cosines and sines of its angles. */
+template <bool Interleaved> struct Turn {
+    Eight straight, cross;
+
+    __device__ __forceinline__ Turn(const __nv_bfloat16 *weight, const float *cosines, int half, bool turns,
+                                    int first, int second)
+    {
+        straight = {{two(1.f, 1.f), two(1.f, 1.f)}, {two(1.f, 1.f), two(1.f, 1.f)}};
+        cross = {};
         if (weight) {
-            const float scale = rsqrtf(square / task.depth + task.epsilon);
-            const Piece wa = load_piece(weight + first), wb = load_piece(weight + second);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                a.e[i] *= scale * wa.e[i], b.e[i] *= scale * wb.e[i];
+            const uint2 a = *reinterpret_cast<const uint2 *>(weight + first);
+            const uint2 b = *reinterpret_cast<const uint2 *>(weight + second);
+            straight = {{widen_pair(a.x), widen_pair(a.y)}, {widen_pair(b.x), widen_pair(b.y)}};
         }
-        if (kind != 2 && unit < turned && placed) {
-            const float *row = task.table + position * task.rotary + 4 * unit;
-            const float4 c4 = *reinterpret_cast<const float4 *>(row);
-            const float4 s4 = *reinterpret_cast<const float4 *>(row + task.rotary / 2);
-            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-            if (task.interleaved) {
-                Piece *both[2] = {&a, &b};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float &x = both[i / 2]->e[2 * (i & 1)], &y = both[i / 2]->e[2 * (i & 1) + 1];
-                    const float turned_x = x * c[i] - y * s[i];
-                    y = y * c[i] + x * s[i], x = turned_x;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float turned_x = a.e[i] * c[i] - b.e[i] * s[i];
-                    b.e[i] = b.e[i] * c[i] + a.e[i] * s[i], a.e[i] = turned_x;
-                }
-            }
-        }
-        if (!placed) /* a padding row: zeros, and nothing enters the cache */
-            a = Piece{}, b = Piece{};
-        if (kind == 0 || (kind == 1 && task.k_out)) {
-            const int count = kind == 0 ? task.heads : task.kv_heads;
-            __nv_bfloat16 *to = (kind == 0 ? task.q_out : task.k_out) +
-                                ((long long)token * count + head) * task.depth;
-            store_piece(to + first, a), store_piece(to + second, b);
-        }
-        if (kind != 0 && placed && slot >= 0 && slot < task.slot_count) {
-            const CacheLayout &cache = kind == 1 ? task.key_cache : task.value_cache;
-            const long long page = slot / task.page_size;
-            const long long at = page * cache.page_stride +
-                                 (slot - page * task.page_size) * cache.slot_stride +
-                                 head * cache.head_stride;
-            if (task.eight_bit) {
-                uint8_t *to = static_cast<uint8_t *>(cache.base) + at;
-                const float scale = kind == 1 ? task.key_scale : task.value_scale;
-                store_piece_e4m3(to + first, a, scale), store_piece_e4m3(to + second, b, scale);
-            } else {
-                __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(cache.base) + at;
-                store_piece(to + first, a), store_piece(to + second, b);
-            }
+        if (!turns)
+            return;
+        const float4 c = *reinterpret_cast<const float4 *>(cosines);
+        const float4 s = *reinterpret_cast<const float4 *>(cosines + half);
+        if constexpr (Interleaved) {
+            /* pair (x, y): x' = x wx c - y wy s, y' = y wy c + x wx s; pairs 0, 1 in a, 2, 3 in b */
+            cross.a[0] = multiply(swapped(straight.a[0]), two(-s.x, s.x));
+            cross.a[1] = multiply(swapped(straight.a[1]), two(-s.y, s.y));
+            cross.b[0] = multiply(swapped(straight.b[0]), two(-s.z, s.z));
+            cross.b[1] = multiply(swapped(straight.b[1]), two(-s.w, s.w));
+            straight.a[0] = multiply(straight.a[0], two(c.x, c.x));
+            straight.a[1] = multiply(straight.a[1], two(c.y, c.y));
+            straight.b[0] = multiply(straight.b[0], two(c.z, c.z));
+            straight.b[1] = multiply(straight.b[1], two(c.w, c.w));
+        } else {
+            const Two low = two(c.x, c.y), high = two(c.z, c.w);
+            cross.a[0] = multiply(straight.b[0], two(-s.x, -s.y));
+            cross.a[1] = multiply(straight.b[1], two(-s.z, -s.w));
+            cross.b[0] = multiply(straight.a[0], two(s.x, s.y));
+            cross.b[1] = multiply(straight.a[1], two(s.z, s.w));
+            straight.a[0] = multiply(straight.a[0], low), straight.a[1] = multiply(straight.a[1], high);
+            straight.b[0] = multiply(straight.b[0], low), straight.b[1] = multiply(straight.b[1], high);
         }
     }
+
+    __device__ __forceinline__ Eight apply(const Eight &x, bool turns, float scale) const
+    {
+        Eight y;
+        const Two scales = two(scale, scale);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            y.a[i] = multiply(x.a[i], straight.a[i]), y.b[i] = multiply(x.b[i], straight.b[i]);
+            if (turns) { /* elsewhere cross is 0, but 0 times an infinity is not */
+                y.a[i] = multiply_add(Interleaved ? swapped(x.a[i]) : x.b[i], cross.a[i], y.a[i]);
+                y.b[i] = multiply_add(Interleaved ? swapped(x.b[i]) : x.a[i], cross.b[i], y.b[i]);
+            }
+            y.a[i] = multiply(y.a[i], scales), y.b[i] = multiply(y.b[i], scales);
+        }
+        return y;
+    }
+};
+
+/* `Lanes` lanes share a head; a CTA takes one token's query heads, key heads and,
+ * with a cache, value heads, or every gridDim.y-th round of them. What does not
+ * depend on the head (the products of weight and cosine or sine) is done once
+ * per lane and kind, and `Batch` heads of a lane are fetched before the first
+ * is worked on. */
+template <int Lanes, int Batch, bool Interleaved>
+__global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(const __grid_constant__ RotateTask task)
+{
+    constexpr int kGroups = kThreads / Lanes;
+    constexpr unsigned kSharing = Lanes == 32 ? 0xffffffffu : (1u << (Lanes % 32)) - 1;
+    const unsigned sharing = kSharing << (threadIdx.x % 32 / Lanes * Lanes); /* the lanes of this head */
+    const int token = blockIdx.x;
+    const int unit = threadIdx.x % Lanes;
+    const bool live = 8 * unit < task.depth;
+    const bool turns = 8 * unit < task.rotary;
+    const int first = !Interleaved && turns ? 4 * unit : 8 * unit;
+    const int second = !Interleaved && turns ? first + task.rotary / 2 : first + 4;
+    const int step = gridDim.y * kGroups, group = blockIdx.y * kGroups + threadIdx.x / Lanes;
+    const long long position = task.positions[token];
+    const bool placed = position >= 0 && position < task.table_rows;
+    const float *cosines = task.table + position * task.rotary + 4 * unit;
+
+    /* Works on heads h = begin, begin + step, ... below count, the first at `source`: turns them
+     * (nullptr: leaves them as they are) and hands each to store(h, a, b). */
+    const auto run = [&](int begin, int count, const __nv_bfloat16 *source, int head_stride, const auto *turn,
+                         bool normalise, auto store) {
+        const __nv_bfloat16 *at_first = source + (long long)begin * head_stride + first;
+        const __nv_bfloat16 *at_second = at_first + (second - first);
+        const long long ahead = (long long)step * head_stride;
+        for (int head = begin; head < count; head += Batch * step) {
+            uint2 raw[Batch][2];
+#pragma unroll
+            for (int i = 0; i < Batch; ++i) {
+                raw[i][0] = raw[i][1] = make_uint2(0, 0);
+                if (live && head + i * step < count) {
+                    raw[i][0] = *reinterpret_cast<const uint2 *>(at_first);
+                    raw[i][1] = *reinterpret_cast<const uint2 *>(at_second);
+                }
+                at_first += ahead, at_second += ahead;
+            }
+#pragma unroll
+            for (int i = 0; i < Batch; ++i) {
+                if (head + i * step >= count)
+                    break;
+                Eight x = {{widen_pair(raw[i][0].x), widen_pair(raw[i][0].y)},
+                           {widen_pair(raw[i][1].x), widen_pair(raw[i][1].y)}};
+                if (turn) {
+                    float scale = 1.f;
+                    if (normalise) {
+                        const Two square_two = multiply_add(
+                            x.b[1], x.b[1],
+                            multiply_add(x.b[0], x.b[0], multiply_add(x.a[1], x.a[1], multiply(x.a[0], x.a[0]))));
+                        float square = both(square_two).x + both(square_two).y;
+#pragma unroll
+                        for (int offset = Lanes / 2; offset > 0; offset /= 2)
+                            square += __shfl_xor_sync(sharing, square, offset, Lanes);
+                        scale = rsqrtf(square * task.inverse_depth + task.epsilon);
+                    }
+                    x = turn->apply(x, turns, scale);
+                }
+                if (live)
+                    store(head + i * step, as_piece(x.a), as_piece(x.b));
+            }
+        }
+    };
+
+    if (!placed) { /* a padding row: zeros, and nothing enters the cache */
+        const Piece zero{};
+        for (int head = group; live && head < task.heads; head += step) {
+            __nv_bfloat16 *to = task.q_out + ((long long)token * task.heads + head) * task.depth;
+            store_piece(to + first, zero), store_piece(to + second, zero);
+        }
+        for (int head = group; live && task.k_out && head < task.kv_heads; head += step) {
+            __nv_bfloat16 *to = task.k_out + ((long long)token * task.kv_heads + head) * task.depth;
+            store_piece(to + first, zero), store_piece(to + second, zero);
+        }
+        return;
+    }
+    if (group < task.heads) {
+        const Turn<Interleaved> turn(live ? task.q_weight : nullptr, cosines, task.rotary / 2, turns, first,
+                                     second);
+        __nv_bfloat16 *out = task.q_out + (long long)token * task.heads * task.depth;
+        run(group, task.heads, task.q + token * task.q_token, task.q_head, &turn, task.q_weight != nullptr,
+            [&](int head, const Piece &a, const Piece &b) {
+                store_piece(out + head * task.depth + first, a), store_piece(out + head * task.depth + second, b);
+            });
+    }
+    /* where the token's keys and values go in the caches; -1: nowhere */
+    long long page = -1, place = 0;
+    if (task.v) {
+        const long long slot = task.slots[token];
+        if (slot >= 0 && slot < task.slot_count)
+            page = slot / task.page_size, place = slot - page * task.page_size;
+    }
+    const auto cache = [&](const CacheLayout &to, int head, float scale, const Piece &a, const Piece &b) {
+        if (page < 0)
+            return;
+        const long long at = page * to.page_stride + place * to.slot_stride + head * to.head_stride;
+        if (task.eight_bit) {
+            uint8_t *row = static_cast<uint8_t *>(to.base) + at;
+            store_piece_e4m3(row + first, a, scale), store_piece_e4m3(row + second, b, scale);
+        } else {
+            __nv_bfloat16 *row = static_cast<__nv_bfloat16 *>(to.base) + at;
+            store_piece(row + first, a), store_piece(row + second, b);
+        }
+    };
+    /* keys follow the queries in the rounds, values the keys */
+    const auto first_after = [&](int before) { return group >= before ? group - before : step - 1 - (before - group - 1) % step; };
+    int begin = first_after(task.heads);
+    if (begin < task.kv_heads) {
+        const Turn<Interleaved> turn(live ? task.k_weight : nullptr, cosines, task.rotary / 2, turns, first,
+                                     second);
+        __nv_bfloat16 *out =
+            task.k_out ? task.k_out + (long long)token * task.kv_heads * task.depth : nullptr;
+        run(begin, task.kv_heads, task.k + token * task.k_token, task.k_head, &turn, task.k_weight != nullptr,
+            [&](int head, const Piece &a, const Piece &b) {
+                if (out)
+                    store_piece(out + head * task.depth + first, a), store_piece(out + head * task.depth + second, b);
+                cache(task.key_cache, head, task.key_scale, a, b);
+            });
+    }
+    begin = first_after(task.heads + task.kv_heads);
+    if (task.v && begin < task.kv_heads && page >= 0)
+        run(begin, task.kv_heads, task.v + token * task.v_token, task.v_head,
+            static_cast<const Turn<Interleaved> *>(nullptr), false,
+            [&](int head, const Piece &a, const Piece &b) { cache(task.value_cache, head, task.value_scale, a, b); });
+}
+
+template <int Lanes, int Batch> void launch_batch(camblas_cuda_context *context, const RotateTask &task, int parts)
+{
+    const dim3 grid(task.tokens, parts);
+    if (task.interleaved)
+        rotate_kernel<Lanes, Batch, true><<<grid, kThreads, 0, context->stream>>>(task);
+    else
+        rotate_kernel<Lanes, Batch, false><<<grid, kThreads, 0, context->stream>>>(task);
 }
 
 template <int Lanes> void launch(camblas_cuda_context *context, const RotateTask &task)
 {
-    const long long items =
-        (long long)task.tokens * (task.heads + (task.v ? 2 : 1) * task.kv_heads);
-    const long long blocks = (items + kThreads / Lanes - 1) / (kThreads / Lanes);
-    rotate_kernel<Lanes><<<unsigned(blocks < (1 << 30) ? blocks : (1 << 30)), kThreads, 0,
-                           context->stream>>>(task);
+    /* Enough tokens to fill the chip: a CTA takes all heads of a token. Fewer: a head per lane, and
+     * as many CTAs per token as that takes. */
+    const int all_heads = task.heads + (task.v ? 2 : 1) * task.kv_heads;
+    const int groups = kThreads / Lanes, rounds = (all_heads + groups - 1) / groups;
+    if (task.tokens < 2 * context->sm_count)
+        launch_batch<Lanes, 1>(context, task, rounds);
+    else
+        launch_batch<Lanes, kBatch>(context, task, 1);
 }
 
 inline bool misaligned(const void *pointer, unsigned bytes)
@@ -250,18 +398,18 @@ extern "C" int camblas_cuda_qk_norm_rope(
         for (const void *pointer : pieces)
             bad = bad || heads::misaligned(pointer, 8);
         for (int i = 0; i < (cached ? 6 : 4) && !bad; ++i)
-            bad = strides[i] % 4 != 0;
+            bad = strides[i] % 4 != 0 || (i % 2 == 1 && (strides[i] < INT_MIN || strides[i] > INT_MAX));
         if (bad || q_out == q || q_out == k || q_out == v || (k_out && (k_out == q || k_out == k)) ||
             q_out == k_out)
             return host::fail(context, "invalid head rotation operands", 1);
         heads::RotateTask task{};
         task.tokens = tokens, task.heads = heads_count, task.kv_heads = kv_heads;
         task.depth = depth, task.rotary = rotary, task.table_rows = table_rows;
-        task.interleaved = interleaved, task.epsilon = epsilon;
+        task.interleaved = interleaved, task.epsilon = epsilon, task.inverse_depth = 1.f / depth;
         task.q = static_cast<const __nv_bfloat16 *>(q);
         task.k = static_cast<const __nv_bfloat16 *>(k);
-        task.q_token = strides[0], task.q_head = strides[1];
-        task.k_token = strides[2], task.k_head = strides[3];
+        task.q_token = strides[0], task.q_head = int(strides[1]);
+        task.k_token = strides[2], task.k_head = int(strides[3]);
         task.q_weight = static_cast<const __nv_bfloat16 *>(q_weight);
         task.k_weight = static_cast<const __nv_bfloat16 *>(k_weight);
         task.positions = static_cast<const int64_t *>(positions);
@@ -272,7 +420,7 @@ extern "C" int camblas_cuda_qk_norm_rope(
         if (cached) {
             task.eight_bit = cache_type == 3;
             task.v = static_cast<const __nv_bfloat16 *>(v);
-            task.v_token = strides[4], task.v_head = strides[5];
+            task.v_token = strides[4], task.v_head = int(strides[5]);
             task.slots = static_cast<const int64_t *>(slots);
             task.key_cache = {key_cache, strides[6], strides[7], strides[8]};
             task.value_cache = {value_cache, strides[9], strides[10], strides[11]};

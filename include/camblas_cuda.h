@@ -490,7 +490,8 @@ int camblas_cuda_reduce_groups(camblas_cuda_context *context, int tokens, int ch
  * {q token, q head, k token, k head, v token, v head, key page, key slot, key
  * head, value page, value slot, value head}, the last eight only with a cache.
  * depth a multiple of 8 up to 256, rotary a multiple of 8 up to depth; q, k, v,
- * outputs 8-byte aligned and their strides multiples of 4; table 16-byte
+ * outputs 8-byte aligned, their strides multiples of 4 and the head strides
+ * below 2^31; table 16-byte
  * aligned; caches aligned to 4 elements and their strides multiples of 4.
  * Outputs overlap no input. */
 int camblas_cuda_qk_norm_rope(camblas_cuda_context *context, int tokens, int heads, int kv_heads,
