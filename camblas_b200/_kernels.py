@@ -929,7 +929,7 @@ class Int4Weight:
     BF16 or FP32 ``[outputs, inner/group]`` with groups of 32, 64 or 128 inputs; ``zero`` uint8
     0..15 of the same shape, or ``None`` for 8 throughout. Element ``(o, k)`` stands for
     ``(code - zero) * scale``. The codes are copied into the order the kernel's lanes read
-    (``camblas_cuda_int4_linear``), outputs padded to 16 and inputs to 64; the arguments are not
+    (``camblas_cuda_int4_linear``), outputs padded to 64 and inputs to 128; the arguments are not
     kept.
     """
 
@@ -941,44 +941,50 @@ class Int4Weight:
                  and scale.dim() == 2 and scale.shape[0] == outputs and scale.shape[1] >= 1
                  and inner % scale.shape[1] == 0 and inner // scale.shape[1] in (32, 64, 128),
                  "scale must be BF16 or FP32 [outputs, inner/group] with groups of 32, 64 or 128")
-        _require(outputs <= _INT_MAX - 16 and inner <= _INT_MAX - 64, "LP64 dimension overflow")
-        self.outputs, self.inner, self.group = outputs, inner, inner // scale.shape[1]
-        tiles, blocks = (outputs + 15) // 16, (inner + 63) // 64
-
-        def tiled(values):  # [outputs, groups] -> [tile, group, g, r], padded with zeros
-            padded = torch.zeros((tiles * 16, values.shape[1]), dtype=values.dtype, device=values.device)
-            padded[:outputs] = values
-            return padded.view(tiles, 2, 8, -1).permute(0, 3, 2, 1).contiguous()
-
+        _require(outputs <= _INT_MAX - 64 and inner <= _INT_MAX - 128, "LP64 dimension overflow")
+        group = inner // scale.shape[1]
         if zero is not None:
             _require(zero.device == codes.device and zero.dtype == torch.uint8 and zero.shape == scale.shape
                      and int(zero.max()) <= 15, "zero must be uint8 0..15 of the shape of scale")
-            zero = tiled(zero)
-        self.scale, self.zero = tiled(scale.detach()), zero
+        self.outputs, self.inner, self.group = outputs, inner, group
         self.scale_type = 0 if scale.dtype == torch.float32 else 2
-        words = torch.zeros((tiles, blocks, 8, 4, 2, 2), dtype=torch.int32, device=codes.device)
-        padded = torch.zeros((tiles * 16, blocks * 32), dtype=torch.uint8, device=codes.device)
+        self.zeros = 0 if zero is None else 1
+        tiles, units = 4 * ((outputs + 63) // 64), (inner + 127) // 128
+
+        def tiled(values):  # [outputs, groups] -> bytes [tile, unit, (group, g, r)], padded with zeros
+            padded = torch.zeros((tiles * 16, units * (128 // group)), dtype=values.dtype, device=values.device)
+            padded[:outputs, :values.shape[1]] = values
+            padded = padded.view(tiles, 2, 8, units, -1).permute(0, 3, 4, 2, 1).contiguous()
+            return padded.view(torch.uint8).view(tiles, units, -1)
+
+        words = torch.zeros((tiles, 2 * units, 8, 4, 2, 2), dtype=torch.int32, device=codes.device)
+        padded = torch.zeros((tiles * 16, units * 64), dtype=torch.uint8, device=codes.device)
         padded[:outputs, :inner // 2] = codes
-        # [tile, r, g, block, h, t, m, j // 2], a byte holding j % 2 = 0 (low nibble) and 1
-        parts = padded.view(tiles, 2, 8, blocks, 2, 4, 2, 2)
+        # [tile, r, g, half unit, h, t, m, j // 2], a byte holding j % 2 = 0 (low nibble) and 1
+        parts = padded.view(tiles, 2, 8, 2 * units, 2, 4, 2, 2)
         for r in range(2):
             for pair in range(2):
-                byte = parts[:, r, ..., pair].permute(0, 2, 1, 4, 3, 5).int()  # [tile, block, g, t, h, m]
+                byte = parts[:, r, ..., pair].permute(0, 2, 1, 4, 3, 5).int()  # [tile, half, g, t, h, m]
                 at = 4 * (r + 2 * pair)
                 words |= ((byte & 15) << at) | ((byte >> 4) << (at + 16))
-        self.codes = words
+        pieces = [words.view(torch.uint8).view(tiles, units, 1024), tiled(scale.detach())]
+        if zero is not None:
+            pieces.append(tiled(zero))
+        # [tile, unit, bytes] -> [block of four tiles, unit, tile, bytes]
+        self.packed = torch.cat(pieces, dim=2).view(tiles // 4, 4, units, -1).transpose(1, 2).contiguous()
 
 
 def int4_linear(x, weight, bias=None, residual=None):
     """``x @ W.T (+ bias) (+ residual)`` for a 4-bit ``Int4Weight``, BF16 ``[..., outputs]``.
 
-    The products are of exact operands (whole numbers against BF16), sums and scales FP32, with
-    one rounding. Made for the few token rows of decoding, where reading the weight is the cost:
-    up to 32 rows read it once, more rows once per 32.
+    The products are of exact operands (whole numbers against the inputs; only inputs below 2^-21
+    of the largest of their 128 are rounded), sums and scales FP32, with one rounding. An input
+    that is not finite makes its token's outputs NaN. Made for the few token rows of decoding,
+    where reading the weight is the cost: up to 64 rows read it once, more rows once per 64.
     """
     _require(isinstance(weight, Int4Weight), "weight must be an Int4Weight")
     _refuse_gradient(x, bias, residual)
-    inner, outputs, index = weight.inner, weight.outputs, weight.codes.get_device()
+    inner, outputs, index = weight.inner, weight.outputs, weight.packed.get_device()
     _require(x.get_device() == index and x.dtype is torch.bfloat16 and x.dim() >= 1 and x.shape[-1] == inner,
              "int4_linear requires CUDA BF16 x [..., inner] on the weight's device")
     lead = x.shape[:-1]
@@ -1002,10 +1008,12 @@ def int4_linear(x, weight, bias=None, residual=None):
         ldr = r2.stride(0) if rows > 1 else outputs
     out = x.new_empty((*lead, outputs))
     if rows:
-        _native.context(index).call(
-            "int4_linear", rows, inner, outputs, weight.group, x2.data_ptr(), ldx if rows > 1 else inner,
-            weight.codes.data_ptr(), weight.scale_type, weight.scale.data_ptr(), _address(weight.zero),
-            _address(bias), _address(r2), ldr, out.data_ptr(), outputs)
+        native = _native.context(index)
+        size = native.workspace_bytes("int4_linear", rows, inner, weight.group)
+        workspace = x.new_empty((size // 2,))  # of the stream's pool, or of the capturing graph's own
+        native.call("int4_linear", rows, inner, outputs, weight.group, x2.data_ptr(), ldx if rows > 1 else inner,
+                    weight.packed.data_ptr(), weight.scale_type, weight.zeros, _address(bias), _address(r2), ldr,
+                    workspace.data_ptr(), size, out.data_ptr(), outputs)
     return out
 
 

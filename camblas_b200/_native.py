@@ -125,9 +125,10 @@ _SIGNATURES = {
          ct.c_size_t, _P],
         _I,
     ),
+    "int4_linear_workspace": ([_P, _I, _I, _I], ct.c_size_t),
     "int4_linear": (
-        [_P, _I, _I, _I, _I, _P, ct.c_longlong, _P, _I, _P, _P, _P, _P, ct.c_longlong, _P,
-         ct.c_longlong],
+        [_P, _I, _I, _I, _I, _P, ct.c_longlong, _P, _I, _I, _P, _P, ct.c_longlong, _P,
+         ct.c_size_t, _P, ct.c_longlong],
         _I,
     ),
     "route_experts": (

@@ -111,7 +111,7 @@ int create_here(int device, void *stream, camblas_cuda_context **out)
     if (status == 0) {
         what = "kernel attributes";
         status = host::prepare_kernels() | fp8::prepare_kernels() | fp8::prepare_wide_kernels() |
-                 prepare_rms_kernels() | attend::prepare_kernels();
+                 prepare_rms_kernels() | attend::prepare_kernels() | nibble::prepare_kernels();
     }
     if (status != 0) {
         cudaGetLastError();

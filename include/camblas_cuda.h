@@ -533,20 +533,27 @@ int camblas_cuda_paged_attention(camblas_cuda_context *context, int batch, int h
  * inner] . W^T (+ bias) (+ residual), BF16, where W[o,k] = (code - zero) *
  * scale, code and zero whole numbers 0..15 (zero 8 when zeros is NULL), scale
  * and zero of output o and group k / group. Products of exact operands, FP32
- * sums, scales applied in FP32, one rounding. scale_type 0 FP32, 2 BF16. codes,
- * scales and zeros in the order that the Int4Weight class of the Python layer
- * produces: codes [tiles of 16 outputs][blocks of 64 inputs][32 lanes 4g +
- * t][4 words 2h + m], word nibble r + 2 (j / 2) + 4 (j % 2) = code of output
- * 16 tile + g + 8r and input 64 block + 32h + 8t + 4m + j; scales, and zeros
- * (one byte each), [tiles][inner / group][8 g][2 r]; outputs padded to 16,
- * inputs to 64, with scale zero. group 32, 64 or 128, inner a multiple of it;
- * rows <= 65535; x 16-byte aligned, ldx a multiple of 8, codes 16-byte aligned.
- * Above a few dozen rows the weights are read once per 32 rows. */
+ * sums, scales applied in FP32, one rounding (of x, what lies below 2^-21 of the
+ * largest of its 128 inputs keeps an absolute error of 2^-25 of that; an element
+ * that is not finite makes its token's outputs NaN). scale_type 0 FP32, 2 BF16;
+ * zeros 1 when the weights hold zero points. weights is what the Int4Weight class
+ * of the Python layer produces: [blocks of 64 outputs][units of 128 inputs][4
+ * tiles of 16 outputs], a tile being 1024 bytes of codes [2 halves][32 lanes 4g +
+ * t][4 words 2h + m], word nibble r + 2 (j / 2) + 4 (j % 2) = code of output 16
+ * tile + g + 8r and input 64 half + 32h + 8t + 4m + j, then scales [128 / group][8
+ * g][2 r], then zero points of one byte in the same order; outputs padded to 64,
+ * inputs to 128, with scale zero. group 32, 64 or 128, inner a multiple of it; rows <= 65535; x
+ * 16-byte aligned, ldx a multiple of 8, weights 16-byte aligned. workspace: device
+ * memory of at least camblas_cuda_int4_linear_workspace bytes (0 for invalid
+ * sizes), 16-byte aligned, used by this call only until it has run. Up to 64
+ * rows the weights are read once, more rows read them once per 64. */
+size_t camblas_cuda_int4_linear_workspace(const camblas_cuda_context *context, int rows, int inner,
+                                          int group);
 int camblas_cuda_int4_linear(camblas_cuda_context *context, int rows, int inner, int outputs,
-                             int group, const void *x, long long ldx, const void *codes,
-                             int scale_type, const void *scales, const void *zeros,
-                             const void *bias, const void *residual, long long ldr, void *out,
-                             long long ldo);
+                             int group, const void *x, long long ldx, const void *weights,
+                             int scale_type, int zeros, const void *bias, const void *residual,
+                             long long ldr,
+                             void *workspace, size_t workspace_bytes, void *out, long long ldo);
 
 /* Router of a mixture of experts. score = softmax(logits) over a token's
  * experts, or 1 / (1 + exp(-logits)) when sigmoid; rank = score + bias

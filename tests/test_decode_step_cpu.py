@@ -40,13 +40,14 @@ def test_null_context_is_a_status_not_a_crash():
                           null, 0, null, null, 0, 1, 1.0, 1.0, null)),
         ("paged_attention", (1, 1, 1, 64, 1.0, null, 2, null, null, strides, 1, 1, 1.0, 1.0, null, 1, null, 0, 0,
                              null, 0, null)),
-        ("int4_linear", (1, 32, 16, 32, null, 32, null, 2, null, null, null, null, 0, null, 16)),
+        ("int4_linear", (1, 32, 16, 32, null, 32, null, 2, 0, null, null, 0, null, 0, null, 16)),
         ("route_experts", (0, 1, 8, 2, 0, 1, 1, 1, 1.0, null, 8, null, null, null)),
     )
     for name, arguments in calls:
         assert getattr(library, "camblas_cuda_" + name)(None, *arguments) < 0
         assert b"missing context" in library.camblas_cuda_error(None)
     assert library.camblas_cuda_paged_attention_workspace(None, 1, 8, 8, 128, 2, 16, 4, 0, 0) == 0
+    assert library.camblas_cuda_int4_linear_workspace(None, 1, 128, 64) == 0
 
 
 def test_rotary_table_is_formed_in_64_bits():

@@ -351,7 +351,8 @@ def int4_case(gen, outputs, inner, group, zeros, scale_type=BF16):
     (1, 1, 32, 32, False, BF16), (1, 16, 64, 64, True, BF16), (3, 17, 96, 32, True, torch.float32),
     (8, 1280, 4096, 128, False, BF16), (9, 100, 640, 128, True, torch.float32), (16, 33, 1024, 64, False, BF16),
     (17, 250, 224, 32, True, BF16), (32, 512, 2048, 128, False, torch.float32), (33, 48, 512, 64, True, BF16),
-    (70, 1003, 1120, 32, False, BF16), (1, 4096, 14336, 128, True, BF16), (2, 64, 11008, 32, False, torch.float32)])
+    (70, 1003, 1120, 32, False, BF16), (1, 4096, 14336, 128, True, BF16), (2, 64, 11008, 32, False, torch.float32),
+    (3, 17000, 256, 64, True, BF16), (45, 130, 1536, 64, False, BF16), (130, 70, 416, 32, True, torch.float32)])
 def test_int4_linear(gen, rows, outputs, inner, group, zeros, scale_type):
     codes, scale, zero = int4_case(gen, outputs, inner, group, zeros, scale_type)
     weight = _kernels.Int4Weight(codes, scale, zero)
@@ -399,12 +400,18 @@ def test_int4_leaves_its_neighbours_alone(gen):
     weight = _kernels.Int4Weight(codes, scale)
     x = normal(gen, 5, 128).to(BF16)
     out = torch.full((7, 50), float("nan"), device="cuda", dtype=BF16)
-    status, context = raw("int4_linear", 5, 128, 37, 32, pointer(x), 128, pointer(weight.codes), 2,
-                          pointer(weight.scale), None, None, None, 0, pointer(out[1:, 3:]), 50)
+    size = _native.context(0).workspace_bytes("int4_linear", 5, 128, 32)
+    workspace = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+    workspace[size:] = 77
+    status, context = raw("int4_linear", 5, 128, 37, 32, pointer(x), 128, pointer(weight.packed), 2, 0,
+                          None, None, 0, pointer(workspace), size, pointer(out[1:, 3:]), 50)
     assert status == 0, error_text(context)
     assert torch.equal(out[1:6, 3:40], _kernels.int4_linear(x, weight))
     out[1:6, 3:40] = float("nan")
-    assert out.isnan().all()
+    assert out.isnan().all() and (workspace[size:] == 77).all()
+    status, context = raw("int4_linear", 5, 128, 37, 32, pointer(x), 128, pointer(weight.packed), 2, 0,
+                          None, None, 0, pointer(workspace), size - 1, pointer(out), 50)
+    assert status < 0 and "workspace" in error_text(context)
 
 
 def test_int4_refusals(gen):
