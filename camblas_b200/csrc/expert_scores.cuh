@@ -8,12 +8,20 @@
  *   largest rank stay;
  *   the `choices` experts of largest r in them are chosen, in descending order;
  *   weight = s (renormalised: s / sum of the chosen s) * scale.
- * Equal ranks go to the lower index. Ranks are compared in FP64: scores of
- * different experts may lie closer than FP32 can tell, and which expert is
- * chosen is a whole number that no tolerance covers. A NaN ranks behind every
- * number.
+ * Equal ranks go to the lower index, and a NaN ranks behind every number.
  *
- * One warp per token, expert e on lane e % 32.
+ * Which expert is chosen is a whole number that no tolerance covers, and ranks
+ * may lie closer than FP32 can tell. Without bias and groups the logits
+ * themselves are compared: both scores grow with them. Otherwise the choice is
+ * made on FP32 ranks, whose error is bounded, and made again on FP64 ranks for a
+ * token where two ranks that decide anything lie within that bound (a few
+ * tokens in a thousand; every FP64 exponential costs some forty instructions of a
+ * rate of one in two). The weights are FP64 throughout, which is cheap for the
+ * chosen few: renormalised softmax weights do not need the sum over all.
+ *
+ * One warp per token, expert e on lane e % 32; a round of the choice is a local
+ * maximum and two warp reductions of 32-bit keys that are ordered like the ranks.
+ * Issue bounds the kernel, not its few bytes per token.
  */
 #pragma once
 
@@ -56,7 +64,7 @@ __device__ __forceinline__ double shuffle_xor(double x, int offset)
     return __shfl_xor_sync(0xffffffffu, x, offset);
 }
 
-/* The lane and index of the largest key of the warp, the lowest index among
+/* The key and index of the largest key of the warp, the lowest index among
  * equals; index is an expert number or INT_MAX. */
 __device__ __forceinline__ void warp_best(long long &key, int &index)
 {
@@ -69,131 +77,282 @@ __device__ __forceinline__ void warp_best(long long &key, int &index)
     }
 }
 
+/* Lane j < choices: the j-th expert by FP64 ranks. */
+template <int PerLane>
+__device__ __noinline__ int choose_exactly(const ScoreTask &task, const float (&x)[PerLane], float top)
+{
+    const int lane = threadIdx.x & 31;
+    double score[PerLane], sum = 0;
+    long long key[PerLane];
+#pragma unroll
+    for (int i = 0; i < PerLane; ++i) {
+        score[i] = task.sigmoid ? 1.0 / (1.0 + exp(-double(x[i]))) : exp(double(x[i]) - top);
+        sum += score[i];
+    }
+    if (!task.sigmoid) {
+#pragma unroll
+        for (int offset = 16; offset > 0; offset /= 2)
+            sum += shuffle_xor(sum, offset);
+#pragma unroll
+        for (int i = 0; i < PerLane; ++i)
+            score[i] = sum != 0 ? score[i] / sum : 0.0;
+    }
+#pragma unroll
+    for (int i = 0; i < PerLane; ++i) {
+        const int e = i * 32 + lane;
+        key[i] = e < task.experts ? order_of(score[i] + (task.bias ? double(task.bias[e]) : 0.0)) : kRemoved;
+    }
+    if (task.groups > 1) {
+        const int size = task.experts / task.groups;
+        long long mine = kRemoved; /* lane g: the rank of group g */
+        for (int group = 0; group < task.groups; ++group) {
+            long long first = kRemoved, second = kRemoved;
+#pragma unroll
+            for (int i = 0; i < PerLane; ++i) {
+                const int e = i * 32 + lane;
+                if (e >= group * size && e < (group + 1) * size) {
+                    if (key[i] > first)
+                        second = first, first = key[i];
+                    else if (key[i] > second)
+                        second = key[i];
+                }
+            }
+#pragma unroll
+            for (int offset = 16; offset > 0; offset /= 2) {
+                const long long a = __shfl_xor_sync(0xffffffffu, first, offset);
+                const long long b = __shfl_xor_sync(0xffffffffu, second, offset);
+                const long long lower = a < first ? a : first;
+                first = a > first ? a : first;
+                second = second > b ? second : b;
+                second = second > lower ? second : lower;
+            }
+            const auto value = [](long long k) {
+                return k <= kNan ? double(NAN) : __longlong_as_double(k < 0 ? k ^ 0x7fffffffffffffffll : k);
+            };
+            const long long rank = order_of(size > 1 ? value(first) + value(second) : value(first));
+            if (lane == group)
+                mine = rank;
+        }
+        unsigned keep = 0;
+        for (int round = 0; round < task.kept; ++round) {
+            long long best = mine;
+            int at = mine == kRemoved ? INT_MAX : lane;
+            warp_best(best, at);
+            if (at != INT_MAX)
+                keep |= 1u << at;
+            if (lane == at)
+                mine = kRemoved;
+        }
+#pragma unroll
+        for (int i = 0; i < PerLane; ++i) {
+            const int e = i * 32 + lane;
+            if (e < task.experts && !((keep >> (e / size)) & 1))
+                key[i] = kRemoved;
+        }
+    }
+    int mine = 0;
+    for (int round = 0; round < task.choices; ++round) {
+        long long best = kRemoved;
+        int index = INT_MAX;
+#pragma unroll
+        for (int i = 0; i < PerLane; ++i)
+            if (key[i] > best)
+                best = key[i], index = i * 32 + lane;
+        warp_best(best, index);
+        if (lane == round)
+            mine = index;
+#pragma unroll
+        for (int i = 0; i < PerLane; ++i)
+            if (index == i * 32 + lane)
+                key[i] = kRemoved;
+    }
+    return mine;
+}
+
+/* 32-bit keys ordered like FP32 numbers: 0 what was taken out, 1 a NaN. */
+__device__ __forceinline__ unsigned key_of(float x)
+{
+    if (x != x)
+        return 1;
+    const int bits = __float_as_int(x + 0.f);
+    return bits < 0 ? ~unsigned(bits) : unsigned(bits) | 0x80000000u;
+}
+
+__device__ __forceinline__ float rank_of(unsigned key)
+{
+    return key <= 1 ? NAN : __int_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+/* The largest of the warp's keys, the lowest index that has it; taken out. */
+template <int PerLane> __device__ __forceinline__ unsigned take_best(unsigned (&key)[PerLane], int &index)
+{
+    const int lane = threadIdx.x & 31;
+    unsigned best = key[0];
+#pragma unroll
+    for (int i = 1; i < PerLane; ++i)
+        best = max(best, key[i]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    unsigned first = INT_MAX;
+#pragma unroll
+    for (int i = PerLane - 1; i >= 0; --i)
+        if (key[i] == best)
+            first = i * 32 + lane;
+    first = __reduce_min_sync(0xffffffffu, first);
+    index = int(first);
+#pragma unroll
+    for (int i = 0; i < PerLane; ++i)
+        if (first == unsigned(i * 32 + lane))
+            key[i] = 0;
+    return best;
+}
+
+/* Whether a rank that was computed in FP32 is surely larger than another. An FP32 score, at most 1, is
+ * off by less than 2^-18 (an exponential, up to 37 additions of a sum, a division), and its sum with a
+ * bias by a rounding more. */
+__device__ __forceinline__ bool surely_larger(float a, float b)
+{
+    return a - b > 0x1p-17f * (1.f + fabsf(a)); /* false for a NaN and for infinities */
+}
+
 template <int PerLane, typename T>
-__global__ void __launch_bounds__(128) score_kernel(const ScoreTask task)
+__global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ ScoreTask task)
 {
     const int lane = threadIdx.x & 31;
     const int warps = gridDim.x * (blockDim.x / 32);
-    for (int token = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; token < task.tokens;
-         token += warps) {
+    const int size = task.experts / task.groups;
+    for (int token = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; token < task.tokens; token += warps) {
         const T *row = static_cast<const T *>(task.logits) + token * task.ld_logits;
-        double score[PerLane];
-        long long key[PerLane];
+        float x[PerLane];
         float top = -INFINITY;
+        bool broken = false; /* a NaN or +infinity makes every softmax score NaN */
 #pragma unroll
         for (int i = 0; i < PerLane; ++i) {
             const int e = i * 32 + lane;
-            const float x = e < task.experts ? load_logit(row + e) : -INFINITY;
-            score[i] = x;
-            top = fmaxf(top, x);
+            x[i] = e < task.experts ? load_logit(row + e) : -INFINITY;
+            top = fmaxf(top, x[i]);
+            broken = broken || !(x[i] < INFINITY);
         }
-        if (task.sigmoid) {
-#pragma unroll
-            for (int i = 0; i < PerLane; ++i)
-                score[i] = 1.0 / (1.0 + exp(-score[i]));
-        } else {
-#pragma unroll
-            for (int offset = 16; offset > 0; offset /= 2)
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
-            if (top == -INFINITY) /* no expert is open: all scores are zero */
+        if (!task.sigmoid) {
+            top = rank_of(__reduce_max_sync(0xffffffffu, key_of(top)));
+            if (!(top > -INFINITY)) /* no expert is open: all scores are zero */
                 top = 0.f;
-            double sum = 0;
+            broken = __any_sync(0xffffffffu, broken);
+        }
+        unsigned key[PerLane];
+        bool certain = true;
+        const bool by_logits = !task.bias && task.groups == 1;
+        if (by_logits) {
 #pragma unroll
             for (int i = 0; i < PerLane; ++i)
-                score[i] = exp(score[i] - top), sum += score[i];
+                key[i] = i * 32 + lane < task.experts ? (!task.sigmoid && broken ? 1 : key_of(x[i])) : 0;
+        } else {
+            float score[PerLane], sum = 0.f;
 #pragma unroll
-            for (int offset = 16; offset > 0; offset /= 2)
-                sum += shuffle_xor(sum, offset);
-#pragma unroll
-            for (int i = 0; i < PerLane; ++i)
-                score[i] = sum != 0 ? score[i] / sum : 0.0;
-        }
-#pragma unroll
-        for (int i = 0; i < PerLane; ++i) {
-            const int e = i * 32 + lane;
-            key[i] = e < task.experts ? order_of(score[i] + (task.bias ? double(task.bias[e]) : 0.0))
-                                      : kRemoved;
-        }
-        if (task.groups > 1) {
-            const int size = task.experts / task.groups;
-            long long mine = kRemoved; /* lane g: the rank of group g */
-            for (int group = 0; group < task.groups; ++group) {
-                long long first = kRemoved, second = kRemoved;
-#pragma unroll
-                for (int i = 0; i < PerLane; ++i) {
-                    const int e = i * 32 + lane;
-                    if (e >= group * size && e < (group + 1) * size) {
-                        if (key[i] > first)
-                            second = first, first = key[i];
-                        else if (key[i] > second)
-                            second = key[i];
-                    }
-                }
-#pragma unroll
-                for (int offset = 16; offset > 0; offset /= 2) {
-                    const long long a = __shfl_xor_sync(0xffffffffu, first, offset);
-                    const long long b = __shfl_xor_sync(0xffffffffu, second, offset);
-                    const long long lower = a < first ? a : first;
-                    first = a > first ? a : first;
-                    second = second > b ? second : b;
-                    second = second > lower ? second : lower;
-                }
-                const auto value = [](long long k) {
-                    return k <= kNan ? double(NAN)
-                                     : __longlong_as_double(k < 0 ? k ^ 0x7fffffffffffffffll : k);
-                };
-                const long long rank =
-                    order_of(size > 1 ? value(first) + value(second) : value(first));
-                if (lane == group)
-                    mine = rank;
+            for (int i = 0; i < PerLane; ++i) {
+                score[i] = task.sigmoid ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - top);
+                sum += score[i];
             }
-            unsigned keep = 0;
-            for (int round = 0; round < task.kept; ++round) {
-                long long best = mine;
-                int at = mine == kRemoved ? INT_MAX : lane;
-                warp_best(best, at);
-                if (at != INT_MAX)
-                    keep |= 1u << at;
-                if (lane == at)
-                    mine = kRemoved;
+            if (!task.sigmoid) {
+#pragma unroll
+                for (int offset = 16; offset > 0; offset /= 2)
+                    sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+                sum = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+                for (int i = 0; i < PerLane; ++i)
+                    score[i] *= sum;
             }
 #pragma unroll
             for (int i = 0; i < PerLane; ++i) {
                 const int e = i * 32 + lane;
-                if (e < task.experts && !((keep >> (e / size)) & 1))
-                    key[i] = kRemoved;
+                key[i] = e < task.experts ? key_of(score[i] + (task.bias ? task.bias[e] : 0.f)) : 0;
+            }
+            if (task.groups > 1) {
+                unsigned mine = 0; /* lane g: the rank of group g */
+                for (int group = 0; group < task.groups; ++group) {
+                    unsigned members[PerLane];
+#pragma unroll
+                    for (int i = 0; i < PerLane; ++i) {
+                        const int e = i * 32 + lane;
+                        members[i] = e >= group * size && e < (group + 1) * size ? key[i] : 0;
+                    }
+                    int index;
+                    float rank = rank_of(take_best(members, index));
+                    if (size > 1)
+                        rank += rank_of(take_best(members, index));
+                    if (lane == group)
+                        mine = key_of(rank);
+                }
+                unsigned keep = 0;
+                float last = 0.f;
+                unsigned one[1] = {mine};
+                for (int round = 0; round < task.kept; ++round) {
+                    int at;
+                    last = rank_of(take_best(one, at));
+                    keep |= 1u << (at & 31);
+                }
+                if (task.kept < task.groups) { /* twice the bound: a group's rank is a sum of two */
+                    const float next = rank_of(__reduce_max_sync(0xffffffffu, one[0]));
+                    certain = surely_larger(0.5f * last, 0.5f * next);
+                }
+#pragma unroll
+                for (int i = 0; i < PerLane; ++i) {
+                    const int e = i * 32 + lane;
+                    bool kept = false;
+                    for (int group = 0; group < task.groups; ++group)
+                        kept = kept || (((keep >> group) & 1) && e >= group * size && e < (group + 1) * size);
+                    if (!kept)
+                        key[i] = 0;
+                }
             }
         }
-        int my_choice = 0;
-        double my_score = 0;
-        for (int round = 0; round < task.choices; ++round) {
-            long long best = kRemoved;
-            int index = INT_MAX;
-            double held = 0;
+        int mine = 0;
+        if (certain) {
+            float before = INFINITY;
+            for (int round = 0; round < task.choices; ++round) {
+                int index;
+                const float rank = rank_of(take_best(key, index));
+                if (!by_logits)
+                    certain = certain && (round == 0 ? rank == rank : surely_larger(before, rank));
+                before = rank;
+                if (lane == round)
+                    mine = index;
+            }
+            if (!by_logits) { /* the first that was not chosen */
+                unsigned next = 0;
 #pragma unroll
-            for (int i = 0; i < PerLane; ++i)
-                if (key[i] > best)
-                    best = key[i], index = i * 32 + lane, held = score[i];
-            warp_best(best, index);
-            held = __shfl_sync(0xffffffffu, held, index & 31);
-            if (lane == round)
-                my_choice = index, my_score = held;
-#pragma unroll
-            for (int i = 0; i < PerLane; ++i)
-                if (index == i * 32 + lane)
-                    key[i] = kRemoved;
+                for (int i = 0; i < PerLane; ++i)
+                    next = max(next, key[i]);
+                next = __reduce_max_sync(0xffffffffu, next);
+                certain = certain && (next == 0 || surely_larger(before, rank_of(next)));
+            }
         }
-        double total = my_score;
+        if (!certain)
+            mine = choose_exactly<PerLane>(task, x, top);
+        /* the weights of the chosen, lane j the j-th */
+        const bool chosen = lane < task.choices;
+        const double logit = chosen ? double(load_logit(row + mine)) : -INFINITY;
+        double score = task.sigmoid ? 1.0 / (1.0 + exp(-logit)) : exp(logit - top);
+        if (!task.sigmoid && broken)
+            score = NAN;
+        double total = 1.0;
         if (task.renormalise) {
+            total = chosen ? score : 0.0;
 #pragma unroll
             for (int offset = 16; offset > 0; offset /= 2)
                 total += shuffle_xor(total, offset);
-            my_score = total != 0 ? my_score / total : 0.0;
+        } else if (!task.sigmoid) {
+            total = 0.0;
+#pragma unroll
+            for (int i = 0; i < PerLane; ++i)
+                total += exp(double(x[i]) - top);
+#pragma unroll
+            for (int offset = 16; offset > 0; offset /= 2)
+                total += shuffle_xor(total, offset);
         }
-        if (lane < task.choices) {
+        if (chosen) {
             const long long at = (long long)token * task.choices + lane;
-            task.chosen[at] = my_choice;
-            task.weights[at] = float(my_score * double(task.scale));
+            task.chosen[at] = mine;
+            task.weights[at] = float((total != 0 ? score / total : 0.0) * double(task.scale));
         }
     }
 }
