@@ -220,6 +220,11 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Scor
     const int lane = threadIdx.x & 31;
     const int warps = gridDim.x * (blockDim.x / 32);
     const int size = task.experts / task.groups;
+    int group_of[PerLane]; /* exact: (e + 1/2) / size is no nearer than 1 / 2048 to a whole number */
+    const float inverse = 1.f / size;
+#pragma unroll
+    for (int i = 0; i < PerLane; ++i)
+        group_of[i] = int((i * 32 + lane + 0.5f) * inverse);
     for (int token = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; token < task.tokens; token += warps) {
         const T *row = static_cast<const T *>(task.logits) + token * task.ld_logits;
         float x[PerLane];
@@ -268,23 +273,30 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Scor
             }
             if (task.groups > 1) {
                 unsigned mine = 0; /* lane g: the rank of group g */
+#pragma unroll 1
                 for (int group = 0; group < task.groups; ++group) {
-                    unsigned members[PerLane];
+                    unsigned first = 0, second = 0;
 #pragma unroll
                     for (int i = 0; i < PerLane; ++i) {
-                        const int e = i * 32 + lane;
-                        members[i] = e >= group * size && e < (group + 1) * size ? key[i] : 0;
+                        const unsigned k = group_of[i] == group ? key[i] : 0;
+                        second = max(second, min(first, k));
+                        first = max(first, k);
                     }
-                    int index;
-                    float rank = rank_of(take_best(members, index));
-                    if (size > 1)
-                        rank += rank_of(take_best(members, index));
+                    const unsigned best = __reduce_max_sync(0xffffffffu, first);
+                    float rank = rank_of(best);
+                    if (size > 1) {
+                        /* the lane of the largest offers its next, the others their first */
+                        const unsigned owners = __ballot_sync(0xffffffffu, first == best);
+                        const unsigned offer = lane == __ffs(owners) - 1 ? second : first;
+                        rank += rank_of(__reduce_max_sync(0xffffffffu, offer));
+                    }
                     if (lane == group)
                         mine = key_of(rank);
                 }
                 unsigned keep = 0;
                 float last = 0.f;
                 unsigned one[1] = {mine};
+#pragma unroll 1
                 for (int round = 0; round < task.kept; ++round) {
                     int at;
                     last = rank_of(take_best(one, at));
@@ -295,19 +307,15 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Scor
                     certain = surely_larger(0.5f * last, 0.5f * next);
                 }
 #pragma unroll
-                for (int i = 0; i < PerLane; ++i) {
-                    const int e = i * 32 + lane;
-                    bool kept = false;
-                    for (int group = 0; group < task.groups; ++group)
-                        kept = kept || (((keep >> group) & 1) && e >= group * size && e < (group + 1) * size);
-                    if (!kept)
+                for (int i = 0; i < PerLane; ++i)
+                    if (!((keep >> (group_of[i] & 31)) & 1))
                         key[i] = 0;
-                }
             }
         }
         int mine = 0;
         if (certain) {
             float before = INFINITY;
+#pragma unroll 1
             for (int round = 0; round < task.choices; ++round) {
                 int index;
                 const float rank = rank_of(take_best(key, index));
