@@ -98,14 +98,21 @@ __device__ __forceinline__ Visible visible(const AttendTask &task, int length)
     return v;
 }
 
+/* Quotient of numbers that are not negative: the 64-bit division, some hundred instructions, only
+ * where it is needed. */
+__device__ __forceinline__ long long divide(long long a, long long b)
+{
+    return (a | b) >> 32 ? a / b : (long long)(unsigned(a) / unsigned(b));
+}
+
 /* The range of tiles of a worker: `total` in equal parts, the first ones a tile longer. */
 struct Cut {
     long long each;
     long long longer; /* workers with one tile more */
 
     __device__ __forceinline__ Cut(long long total, int workers)
-        : each(total / workers), longer(total % workers)
     {
+        each = divide(total, workers), longer = total - each * workers;
     }
     __device__ __forceinline__ long long start(int worker) const
     {
@@ -114,7 +121,7 @@ struct Cut {
     __device__ __forceinline__ int owner(long long tile) const
     {
         const long long in_longer = longer * (each + 1);
-        return int(tile < in_longer ? tile / (each + 1) : longer + (tile - in_longer) / each);
+        return int(tile < in_longer ? divide(tile, each + 1) : longer + divide(tile - in_longer, each));
     }
 };
 
@@ -313,7 +320,7 @@ template <int Depth, int Blocks, bool Eight> struct Shape {
     static constexpr int kTileBytes = 2 * kTile * kRowBytes; /* keys and values */
     /* The copies in flight on an SM have to cover the latency of HBM at its share of the
      * bandwidth, some 45 KB. */
-    static constexpr int kStages = 3;
+    static constexpr int kStages = kRowBytes >= 512 ? 3 : 2;
     static constexpr int kNoteBytes = 16 * kTile + 16; /* where the rows of a stage lie, which are real */
     static constexpr int kWarpBytes = kStages * (kTileBytes + kNoteBytes);
     static constexpr int kBytes = kWarps * kWarpBytes;
@@ -371,16 +378,16 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
     const long long total = count_tiles(task, global_warp == 0);
     const Cut cut(total, task.workers);
     const long long begin = cut.start(worker);
-    const int count = int(cut.start(worker + 1) - begin);
-    if (count <= 0 || worker >= task.workers)
+    if (worker >= task.workers || begin >= total)
         return;
+    const int count = int(min(cut.start(worker + 1), total) - begin);
     Cursor use;
     {
         long long first;
         int sequence;
         locate(task, begin, sequence, first);
         use.enter(task, sequence, member);
-        const int item = int((begin - first) / use.view.tiles);
+        const int item = int(divide(begin - first, use.view.tiles));
         use.choose(task, item, member);
         use.tile = int(begin - first - (long long)item * use.view.tiles);
     }
@@ -698,30 +705,29 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
 
 /* Adds the pieces of an item that more than one worker took part in, in token
  * order; a programmatic dependent of attend_kernel. blockIdx.x: item and column
- * block, blockIdx.y: 32 * kJoinProducts depths. The warps of a CTA each take a
- * contiguous share of the pieces, kJoinAtOnce in flight; their sums are added
- * through shared memory. */
+ * block. A warp adds `Products` 16-depth products; `parts` warps each take a
+ * contiguous share of the pieces, `AtOnce` in flight, and their sums are added
+ * through shared memory. The products that do not fit a CTA are blockIdx.y's. */
 constexpr int kJoinWarps = 16; /* at most */
-constexpr int kJoinProducts = 2;
-constexpr int kJoinAtOnce = 4;
 
-template <bool Eight>
+template <bool Eight, int Products, int AtOnce>
 __global__ void __launch_bounds__(kJoinWarps * 32)
-    attend_join(const __grid_constant__ AttendTask task, int blocks, int depth_pieces)
+    attend_join(const __grid_constant__ AttendTask task, int blocks, int depth_pieces, int parts)
 {
-    __shared__ float4 shared_sum[kJoinWarps][kJoinProducts][32];
+    __shared__ float4 shared_sum[kJoinWarps][Products][32];
     __shared__ float shared_stats[kJoinWarps][2][8];
-    const int part = threadIdx.x / 32, parts = blockDim.x / 32;
+    const int warp = threadIdx.x / 32, part = warp % parts;
     const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int n = blockIdx.x % blocks, item = blockIdx.x / blocks;
-    const int product = blockIdx.y * kJoinProducts;
+    const int product = (blockIdx.y * (blockDim.x / 32 / parts) + warp / parts) * Products;
     const int slots = task.team * task.teams;
     const int sequence = item / slots, slot = item % slots;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long sequence_first = __ldcg(&task.first_tile[sequence]);
-    const int tiles = int((__ldcg(&task.first_tile[sequence + 1]) - sequence_first) / task.teams);
-    const long long first = sequence_first + (long long)(slot / task.team) * tiles;
+    const long long sequence_end = __ldcg(&task.first_tile[sequence + 1]);
     const Cut cut(__ldcg(&task.first_tile[task.batch]), task.workers);
+    const int tiles = int(divide(sequence_end - sequence_first, task.teams));
+    const long long first = sequence_first + (long long)(slot / task.team) * tiles;
     const int from = cut.owner(first), upto = cut.owner(first + tiles - 1);
     if (from == upto)
         return; /* written whole */
@@ -729,18 +735,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     const int first_place = cut.start(from) < first ? 1 : 0;
     const int share = (upto - from + parts) / parts;
     const int begin = from + part * share, end = min(upto + 1, begin + share);
-    float sum[kJoinProducts][4] = {};
+    float sum[Products][4] = {};
     float top[2] = {-INFINITY, -INFINITY}, weight[2] = {0.f, 0.f};
-    for (int base = begin; base < end; base += kJoinAtOnce) {
-        float4 value[kJoinAtOnce][kJoinProducts];
-        float2 stats[kJoinAtOnce][2];
+    for (int base = begin; base < end; base += AtOnce) {
+        float4 value[AtOnce][Products];
+        float2 stats[AtOnce][2];
 #pragma unroll
-        for (int i = 0; i < kJoinAtOnce; ++i) {
+        for (int i = 0; i < AtOnce; ++i) {
             const int worker = min(base + i, end - 1);
             const long long piece =
                 (2ll * (worker * task.team + member) + (worker == from ? first_place : 0)) * blocks + n;
 #pragma unroll
-            for (int c = 0; c < kJoinProducts; ++c)
+            for (int c = 0; c < Products; ++c)
                 value[i][c] = __ldcg(&task.pieces[(piece * depth_pieces + product + c) * 32 + lane]);
             stats[i][0] = __ldcg(&task.statistics[piece * 8 + 2 * t]);
             stats[i][1] = __ldcg(&task.statistics[piece * 8 + 2 * t + 1]);
@@ -749,60 +755,72 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
         for (int h = 0; h < 2; ++h) {
             float best = top[h];
 #pragma unroll
-            for (int i = 0; i < kJoinAtOnce; ++i)
+            for (int i = 0; i < AtOnce; ++i)
                 best = fmaxf(best, stats[i][h].x);
             const float reference = best == -INFINITY ? 0.f : best;
             const float factor = power_of_two(top[h] - reference);
             top[h] = best, weight[h] *= factor;
 #pragma unroll
-            for (int c = 0; c < kJoinProducts; ++c)
+            for (int c = 0; c < Products; ++c)
                 sum[c][h] *= factor, sum[c][h + 2] *= factor;
 #pragma unroll
-            for (int i = 0; i < kJoinAtOnce; ++i) {
+            for (int i = 0; i < AtOnce; ++i) {
                 if (base + i >= end)
                     break;
                 const float share_of = power_of_two(stats[i][h].x - reference);
                 weight[h] += share_of * stats[i][h].y;
 #pragma unroll
-                for (int c = 0; c < kJoinProducts; ++c) {
+                for (int c = 0; c < Products; ++c) {
                     sum[c][h] += share_of * (h == 0 ? value[i][c].x : value[i][c].y);
                     sum[c][h + 2] += share_of * (h == 0 ? value[i][c].z : value[i][c].w);
                 }
             }
         }
     }
+    if (parts > 1) {
 #pragma unroll
-    for (int c = 0; c < kJoinProducts; ++c)
-        shared_sum[part][c][lane] = make_float4(sum[c][0], sum[c][1], sum[c][2], sum[c][3]);
-    if (g == 0)
+        for (int c = 0; c < Products; ++c)
+            shared_sum[warp][c][lane] = make_float4(sum[c][0], sum[c][1], sum[c][2], sum[c][3]);
+        if (g == 0)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            shared_stats[part][0][2 * t + h] = top[h], shared_stats[part][1][2 * t + h] = weight[h];
-    __syncthreads();
-    if (part >= kJoinProducts)
-        return;
-    /* warp c finishes product c */
-    float total[2] = {0.f, 0.f}, result[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < 2; ++h)
+                shared_stats[warp][0][2 * t + h] = top[h], shared_stats[warp][1][2 * t + h] = weight[h];
+        __syncthreads();
+        if (part != 0)
+            return;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float best = -INFINITY;
-        for (int other = 0; other < parts; ++other)
-            best = fmaxf(best, shared_stats[other][0][2 * t + h]);
-        const float reference = best == -INFINITY ? 0.f : best;
-        for (int other = 0; other < parts; ++other) {
-            const float factor = power_of_two(shared_stats[other][0][2 * t + h] - reference);
-            const float4 v = shared_sum[other][part][lane];
-            total[h] += factor * shared_stats[other][1][2 * t + h];
-            result[h] += factor * (h == 0 ? v.x : v.y);
-            result[h + 2] += factor * (h == 0 ? v.z : v.w);
+        for (int h = 0; h < 2; ++h) {
+            float best = -INFINITY;
+            for (int other = 0; other < parts; ++other)
+                best = fmaxf(best, shared_stats[warp + other][0][2 * t + h]);
+            const float reference = best == -INFINITY ? 0.f : best;
+            weight[h] = 0.f;
+#pragma unroll
+            for (int c = 0; c < Products; ++c)
+                sum[c][h] = sum[c][h + 2] = 0.f;
+            for (int other = 0; other < parts; ++other) {
+                const float factor = power_of_two(shared_stats[warp + other][0][2 * t + h] - reference);
+                weight[h] += factor * shared_stats[warp + other][1][2 * t + h];
+#pragma unroll
+                for (int c = 0; c < Products; ++c) {
+                    const float4 v = shared_sum[warp + other][c][lane];
+                    sum[c][h] += factor * (h == 0 ? v.x : v.y);
+                    sum[c][h + 2] += factor * (h == 0 ? v.z : v.w);
+                }
+            }
         }
-        total[h] = total[h] != 0.f ? task.value_scale / total[h] : 0.f;
     }
+    float inverse[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        inverse[h] = weight[h] != 0.f ? task.value_scale / weight[h] : 0.f;
     const int head_block = slot % task.head_blocks;
     const int first_head = slot / task.head_blocks * task.group + (head_block * blocks + n) * 8;
     const int live_heads = task.group - (head_block * blocks + n) * 8;
-    store_heads<Eight>(task.out + ((long long)sequence * task.heads + first_head) * task.depth, task.depth,
-                       live_heads, product + part, result, total);
+#pragma unroll
+    for (int c = 0; c < Products; ++c)
+        store_heads<Eight>(task.out + ((long long)sequence * task.heads + first_head) * task.depth, task.depth,
+                           live_heads, product + c, sum[c], inverse);
 }
 
 /* How one call is cut: kernel instance, CTAs, workspace. */
@@ -873,25 +891,34 @@ void launch(camblas_cuda_context *context, const AttendTask &task, const Plan &p
         <<<plan.grid, kWarps * 32, Shape<Depth, Blocks, Eight>::kBytes, context->stream>>>(task);
 }
 
-template <bool Eight>
-cudaError_t launch_join(camblas_cuda_context *context, const AttendTask &task, const Plan &plan)
+template <bool Eight, int Products, int AtOnce>
+cudaError_t launch_join_of(camblas_cuda_context *context, const AttendTask &task, const Plan &plan, int parts)
 {
-    /* Pieces per item if the lengths are alike; ragged ones give long items many more, so at
-     * least four warps share an item's pieces unless there are items for every warp of the chip. */
-    const int items = task.batch * plan.team * plan.teams;
-    const int expected = plan.grid * kWarps / items + 2;
-    const int parts = expected >= 64 ? 16 : (expected >= 32 ? 8 : (expected > 4 ? 4 : 2));
-    const int depth_pieces = plan.depth_class / 16;
+    const int depth_pieces = plan.depth_class / 16, shares = depth_pieces / Products;
+    const int held = shares < kJoinWarps / parts ? shares : kJoinWarps / parts; /* of a CTA; powers of two */
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(unsigned(items) * plan.blocks, depth_pieces / kJoinProducts);
-    config.blockDim = dim3(parts * 32);
+    config.gridDim = dim3(unsigned(task.batch) * plan.team * plan.teams * plan.blocks, shares / held);
+    config.blockDim = dim3(held * parts * 32);
     config.stream = context->stream;
     cudaLaunchAttribute attribute[1];
     attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attribute;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, attend_join<Eight>, task, plan.blocks, depth_pieces);
+    return cudaLaunchKernelEx(&config, attend_join<Eight, Products, AtOnce>, task, plan.blocks, depth_pieces, parts);
+}
+
+template <bool Eight>
+cudaError_t launch_join(camblas_cuda_context *context, const AttendTask &task, const Plan &plan)
+{
+    /* Pieces per item if the lengths are alike. Few items with many pieces each: a product per warp,
+     * sixteen warps to its pieces. More items: two products per warp and fewer warps per item, so that
+     * the items fit one wave; ragged lengths still give long items more pieces than this. */
+    const int items = task.batch * plan.team * plan.teams;
+    const int expected = plan.grid * kWarps / items + 2;
+    if (expected > 32)
+        return launch_join_of<Eight, 1, 8>(context, task, plan, 16);
+    return launch_join_of<Eight, 2, 4>(context, task, plan, expected > 16 ? 4 : (expected > 4 ? 2 : 1));
 }
 
 template <int Depth, int Blocks, bool Eight> int allow_shared(Shape<Depth, Blocks, Eight>)

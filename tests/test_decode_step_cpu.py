@@ -62,9 +62,9 @@ def test_rotary_table_is_formed_in_64_bits():
     assert _kernels.rotary_table(0, 8, device="cpu").shape == (0, 8)
 
 
-@pytest.mark.parametrize("tiles,per,grid", [((1,), 1, 1), ((1, 1, 1), 8, 296), ((40, 1, 7), 3, 16),
-                                            ((2047,), 8, 296), ((1, 300, 2, 5), 2, 148)])
-def test_equal_ranges_cover_every_tile_once(tiles, per, grid):
+@pytest.mark.parametrize("tiles,per,workers", [((1,), 1, 1), ((1, 1, 1), 8, 296), ((40, 1, 7), 3, 16),
+                                               ((2047,), 8, 296), ((1, 300, 2, 5), 2, 148)])
+def test_equal_ranges_cover_every_tile_once(tiles, per, workers):
     """The cut of the paged attention: ranges, their pieces' places, and the workers an item finds its pieces at."""
     def start(cta):
         return total // grid * cta + min(cta, total % grid)
@@ -74,6 +74,7 @@ def test_equal_ranges_cover_every_tile_once(tiles, per, grid):
         return tile // (each + 1) if tile < longer * (each + 1) else longer + (tile - longer * (each + 1)) // each
 
     total = sum(tiles) * per
+    grid = workers
     written, pieces = {}, {}
     for cta in range(grid):
         tile, end = start(cta), start(cta + 1)
