@@ -12,6 +12,7 @@ raises ``ValueError`` before anything is launched; a native failure raises
 """
 
 import ctypes as ct
+from functools import lru_cache
 
 import torch
 
@@ -19,6 +20,7 @@ from . import _native
 from ._native import algorithm, kernel_family, set_algorithm, stats  # noqa: F401
 
 _INT_MAX = 2**31 - 1
+_INFINITY = float("inf")
 
 
 def _require(condition, message):
@@ -738,47 +740,58 @@ def reduce_groups(grouped, experts, reverse):
 # device is left alone (every entry point works on its context's device).
 
 
+_NO_GRADIENT = "An operand requires a gradient: this operation has none, call it under torch.no_grad()"
+
+
 def _refuse_gradient(*tensors):
     """These operations are for inference; a gradient that was asked for would be lost silently."""
-    if torch.is_grad_enabled():
-        for tensor in tensors:
-            _require(tensor is None or not tensor.requires_grad,
-                     "An operand requires a gradient: this operation has none, call it under torch.no_grad()")
+    for tensor in tensors:
+        if tensor is not None and tensor.requires_grad and torch.is_grad_enabled():
+            raise ValueError(_NO_GRADIENT)
 
 
 def _address(tensor):
     return None if tensor is None else tensor.data_ptr()
 
 
+@lru_cache(maxsize=1024)
+def _stride_array(*strides):
+    """Strides as the C ABI reads them; a serving loop presents the same ones call after call."""
+    return (ct.c_longlong * len(strides))(*strides)
+
+
 def _heads_operand(tensor, index):
     """BF16 ``[rows, heads, depth]`` readable in 8-byte pieces where it lies, else a copy; with its
     row and head strides."""
-    _require(index >= 0 and tensor.get_device() == index and tensor.dtype is torch.bfloat16
-             and tensor.dim() == 3, "Heads must be CUDA BF16 [rows, heads, depth] on one device")
+    if index < 0 or tensor.get_device() != index or tensor.dtype is not torch.bfloat16 or tensor.dim() != 3:
+        raise ValueError("Heads must be CUDA BF16 [rows, heads, depth] on one device")
     row, head, unit = tensor.stride()
-    if unit != 1 or row % 4 or head % 4 or head > _INT_MAX or tensor.data_ptr() % 8:
+    if unit != 1 or (row | head) & 3 or head > _INT_MAX or tensor.data_ptr() & 7:
         tensor = tensor.clone(memory_format=torch.contiguous_format)
         row, head, unit = tensor.stride()
     return tensor, row, head
 
 
-def _check_caches(key_cache, value_cache, index, kv_heads, depth, alignment):
-    """Check a pair of paged caches; return the type code of the C ABI and their six strides."""
-    kind = key_cache.dtype
-    _require((kind is torch.bfloat16 or kind is torch.float8_e4m3fn) and value_cache.dtype is kind
-             and key_cache.get_device() == index and value_cache.get_device() == index,
-             "Caches must be two CUDA tensors on the device of q, both BF16 or both FP8 E4M3")
-    shape = key_cache.shape
-    _require(len(shape) == 4 and value_cache.shape == shape and shape[2] == kv_heads and shape[3] == depth
-             and shape[1] >= 1 and shape[0] <= _INT_MAX and shape[1] <= _INT_MAX,
-             "Caches must be [pages, page size, kv_heads, depth] of one shape that matches the heads")
+def _check_caches(key_cache, value_cache, index, heads, depth, alignment):
+    """Check a pair of paged caches of ``heads`` heads; return the type code of the C ABI, pages, page
+    size and their six strides. ``alignment`` is in elements, a power of two."""
+    kind, shape = key_cache.dtype, key_cache.shape
+    if ((kind is not torch.bfloat16 and kind is not torch.float8_e4m3fn) or value_cache.dtype is not kind
+            or key_cache.get_device() != index or value_cache.get_device() != index):
+        raise ValueError("Caches must be two CUDA tensors on the device of q, both BF16 or both FP8 E4M3")
+    if len(shape) != 4 or value_cache.shape != shape:
+        raise ValueError("Caches must be [pages, page size, kv_heads, depth] of one shape")
+    pages, page_size, kv_heads, width = shape
+    if kv_heads != heads or width != depth or not 1 <= page_size <= _INT_MAX or pages > _INT_MAX:
+        raise ValueError("Cache shape does not match the heads")
     k0, k1, k2, k3 = key_cache.stride()
     v0, v1, v2, v3 = value_cache.stride()
-    elements = alignment // (2 if kind is torch.bfloat16 else 1) - 1  # a power of two less one
-    _require(k3 == 1 and v3 == 1 and not (k0 | k1 | k2 | v0 | v1 | v2) & elements
-             and not (key_cache.data_ptr() | value_cache.data_ptr()) & (alignment - 1),
-             "Caches need unit stride along the depth and aligned rows (16 bytes to read, 4 elements to append)")
-    return (2 if kind is torch.bfloat16 else 3), (k0, k1, k2, v0, v1, v2)
+    code = 2 if kind is torch.bfloat16 else 3
+    if (k3 != 1 or v3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & (alignment - 1)
+            or (key_cache.data_ptr() | value_cache.data_ptr()) & (alignment * (4 - code) - 1)):
+        raise ValueError("Caches need unit stride along the depth and aligned rows "
+                         "(16 bytes to read, 4 elements to append)")
+    return code, pages, page_size, (k0, k1, k2, v0, v1, v2)
 
 
 def rotary_table(positions, rotary, base=10000.0, device="cuda"):
@@ -802,49 +815,55 @@ def _rotate(q, k, v, q_weight, k_weight, epsilon, positions, table, interleaved,
     q, q_row, q_head = _heads_operand(q, index)
     k, k_row, k_head = _heads_operand(k, index)
     tokens, heads, depth = q.shape
-    kv_heads = k.shape[1]
-    _require(k.shape[0] == tokens and k.shape[2] == depth and 8 <= depth <= 256 and depth % 8 == 0
-             and 1 <= heads <= 65536 and 1 <= kv_heads <= 65536 and tokens <= _INT_MAX,
-             "q and k must be [tokens, heads, depth] with one depth, a multiple of 8 up to 256")
+    k_tokens, kv_heads, k_depth = k.shape
+    if (k_tokens != tokens or k_depth != depth or not 8 <= depth <= 256 or depth & 7 or not 1 <= heads <= 65536
+            or not 1 <= kv_heads <= 65536 or tokens > _INT_MAX):
+        raise ValueError("q and k must be [tokens, heads, depth] with one depth, a multiple of 8 up to 256")
     for weight in (q_weight, k_weight):
-        _require(weight is None or (weight.get_device() == index and weight.dtype is torch.bfloat16
-                                    and weight.shape == (depth,) and weight.stride(0) == 1
-                                    and not weight.data_ptr() & 7),
-                 "Norm weights must be contiguous CUDA BF16 [depth]")
-    _require(table.get_device() == index and table.dtype is torch.float32 and table.dim() == 2
-             and table.is_contiguous() and not table.data_ptr() & 15, "table must be contiguous CUDA FP32")
+        if weight is not None and (weight.get_device() != index or weight.dtype is not torch.bfloat16
+                                   or weight.shape != (depth,) or weight.stride(0) != 1 or weight.data_ptr() & 7):
+            raise ValueError("Norm weights must be contiguous CUDA BF16 [depth]")
+    if (table.get_device() != index or table.dtype is not torch.float32 or table.dim() != 2
+            or not table.is_contiguous() or table.data_ptr() & 15):
+        raise ValueError("table must be contiguous CUDA FP32 [positions, rotary]")
     rows, rotary = table.shape
-    _require(rows <= _INT_MAX and rotary <= depth and rotary % 8 == 0,
-             "table must be [positions, rotary], rotary a multiple of 8 up to the depth")
-    _require(0 <= epsilon < float("inf"), "epsilon must be finite and not negative")
-    _require(positions.get_device() == index and positions.dtype is torch.int64
-             and positions.shape == (tokens,) and positions.is_contiguous(),
-             "positions must be contiguous CUDA int64, one per token")
+    if rows > _INT_MAX or rotary > depth or rotary & 7:
+        raise ValueError("rotary, the width of table, must be a multiple of 8 up to the depth")
+    if not 0 <= epsilon < _INFINITY:
+        raise ValueError("epsilon must be finite and not negative")
+    if (positions.get_device() != index or positions.dtype is not torch.int64 or positions.shape != (tokens,)
+            or not positions.is_contiguous()):
+        raise ValueError("positions must be contiguous CUDA int64, one per token")
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    k_out, code, pages, page_size, strides = None, 0, 0, 1, (q_row, q_head, k_row, k_head)
     if key_cache is None:
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-    else:
-        v, v_row, v_head = _heads_operand(v, index)
-        _require(v.shape == k.shape, "v must have the shape of k")
-        code, cache_strides = _check_caches(key_cache, value_cache, index, kv_heads, depth,
-                                            8 if key_cache.dtype is torch.bfloat16 else 4)
-        _require(slots.get_device() == index and slots.dtype is torch.int64 and slots.shape == (tokens,)
-                 and slots.is_contiguous(), "slots must be contiguous CUDA int64, one per token")
-        _require(key_cache.data_ptr() != value_cache.data_ptr() or key_cache.numel() == 0,
-                 "Keys and values need caches of their own")
-        _require(0 < key_scale < float("inf") and 0 < value_scale < float("inf"),
-                 "Cache scales must be positive and finite")
-        pages, page_size = key_cache.shape[0], key_cache.shape[1]
-        strides += (v_row, v_head) + cache_strides
+        if tokens:
+            _native.context(index).call(
+                "qk_norm_rope", tokens, heads, kv_heads, depth, rotary, 1 if interleaved else 0, epsilon,
+                q.data_ptr(), k.data_ptr(), None, _stride_array(q_row, q_head, k_row, k_head),
+                _address(q_weight), _address(k_weight), positions.data_ptr(), table.data_ptr(), rows,
+                q_out.data_ptr(), k_out.data_ptr(), 0, None, None, 0, 1, 1.0, 1.0, None)
+        return q_out, k_out
+    v, v_row, v_head = _heads_operand(v, index)
+    if v.shape != k.shape:
+        raise ValueError("v must have the shape of k")
+    code, pages, page_size, strides = _check_caches(key_cache, value_cache, index, kv_heads, depth, 4)
+    if (slots.get_device() != index or slots.dtype is not torch.int64 or slots.shape != (tokens,)
+            or not slots.is_contiguous()):
+        raise ValueError("slots must be contiguous CUDA int64, one per token")
+    keys, values = key_cache.data_ptr(), value_cache.data_ptr()
+    if keys == values and pages:
+        raise ValueError("Keys and values need caches of their own")
+    if not 0 < key_scale < _INFINITY or not 0 < value_scale < _INFINITY:
+        raise ValueError("Cache scales must be positive and finite")
     if tokens:
         _native.context(index).call(
             "qk_norm_rope", tokens, heads, kv_heads, depth, rotary, 1 if interleaved else 0, epsilon,
-            q.data_ptr(), k.data_ptr(), _address(v), (ct.c_longlong * len(strides))(*strides),
-            _address(q_weight), _address(k_weight), positions.data_ptr(), table.data_ptr(), rows,
-            q_out.data_ptr(), _address(k_out), code, _address(key_cache), _address(value_cache), pages,
-            page_size, key_scale, value_scale, _address(slots))
-    return q_out, k_out
+            q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _stride_array(q_row, q_head, k_row, k_head, v_row, v_head, *strides), _address(q_weight),
+            _address(k_weight), positions.data_ptr(), table.data_ptr(), rows, q_out.data_ptr(), None, code,
+            keys, values, pages, page_size, key_scale, value_scale, slots.data_ptr())
+    return q_out, None
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, epsilon, positions, table, interleaved=False):
@@ -893,20 +912,25 @@ def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, windo
     index = q.get_device()
     q, q_row, q_head = _heads_operand(q, index)
     batch, heads, depth = q.shape
-    _require(key_cache.dim() == 4, "Caches must be [pages, page size, kv_heads, depth]")
-    pages, page_size, kv_heads, _ = key_cache.shape
-    code, cache_strides = _check_caches(key_cache, value_cache, index, kv_heads, depth, 16)
-    _require(kv_heads >= 1 and 1 <= heads <= 65536 and heads % kv_heads == 0 and batch * heads <= _INT_MAX
-             and 8 <= depth <= 256 and depth % (16 if code == 3 else 8) == 0,
-             "paged_attention takes heads a multiple of kv_heads and a depth of a multiple of 8 (E4M3: 16) up to 256")
-    _require(table.get_device() == index and table.dtype is torch.int32 and table.dim() == 2
-             and table.shape[0] == batch, "table must be CUDA int32 [batch, pages of a sequence]")
+    kv_heads = key_cache.shape[2] if key_cache.dim() == 4 else 0
+    code, pages, page_size, strides = _check_caches(key_cache, value_cache, index, kv_heads, depth,
+                                                    8 if key_cache.dtype is torch.bfloat16 else 16)
+    if (kv_heads < 1 or not 1 <= heads <= 65536 or heads % kv_heads or batch * heads > _INT_MAX
+            or not 8 <= depth <= 256 or depth & (15 if code == 3 else 7)):
+        raise ValueError("paged_attention takes heads a multiple of kv_heads and a depth of a multiple of 8 "
+                         "(E4M3: 16) up to 256")
+    if (table.get_device() != index or table.dtype is not torch.int32 or table.dim() != 2
+            or table.shape[0] != batch):
+        raise ValueError("table must be CUDA int32 [batch, pages of a sequence]")
     width = table.shape[1]
     row, column = table.stride()
-    _require(width <= _INT_MAX and row >= 0 and (width <= 1 or column == 1), "table needs unit column stride")
-    _require(lengths.get_device() == index and lengths.dtype is torch.int32 and lengths.shape == (batch,)
-             and lengths.is_contiguous(), "lengths must be contiguous CUDA int32 [batch]")
-    _require(0 <= window <= _INT_MAX and 0 <= sinks <= _INT_MAX, "window and sinks must not be negative")
+    if width > _INT_MAX or row < 0 or (width > 1 and column != 1):
+        raise ValueError("table needs unit column stride")
+    if (lengths.get_device() != index or lengths.dtype is not torch.int32 or lengths.shape != (batch,)
+            or not lengths.is_contiguous()):
+        raise ValueError("lengths must be contiguous CUDA int32 [batch]")
+    if not 0 <= window <= _INT_MAX or not 0 <= sinks <= _INT_MAX:
+        raise ValueError("window and sinks must not be negative")
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if batch:
         native = _native.context(index)
@@ -914,11 +938,11 @@ def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, windo
                                       window, sinks)
         # of the calling stream's pool, or of the capturing graph's own: no other call shares it
         workspace = q.new_empty((size // 2,))
-        strides = (ct.c_longlong * 9)(q_row, q_head, *cache_strides, row)
         native.call("paged_attention", batch, heads, kv_heads, depth, depth ** -0.5 if scale is None else scale,
-                    q.data_ptr(), code, key_cache.data_ptr(), value_cache.data_ptr(), strides, pages, page_size,
-                    key_scale, value_scale, table.data_ptr(), width, lengths.data_ptr(), window, sinks,
-                    workspace.data_ptr(), size, out.data_ptr())
+                    q.data_ptr(), code, key_cache.data_ptr(), value_cache.data_ptr(),
+                    _stride_array(q_row, q_head, *strides, row), pages, page_size, key_scale, value_scale,
+                    table.data_ptr(), width, lengths.data_ptr(), window, sinks, workspace.data_ptr(), size,
+                    out.data_ptr())
     return out
 
 
