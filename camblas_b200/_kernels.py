@@ -1001,7 +1001,7 @@ class Int4Weight:
 def int4_linear(x, weight, bias=None, residual=None):
     """``x @ W.T (+ bias) (+ residual)`` for a 4-bit ``Int4Weight``, BF16 ``[..., outputs]``.
 
-    The products are of exact operands (whole numbers against the inputs; only inputs below 2^-21
+    The products are of exact operands (whole numbers against the inputs; only inputs below 2^-31
     of the largest of their 128 are rounded), sums and scales FP32, with one rounding. An input
     that is not finite makes its token's outputs NaN. Made for the few token rows of decoding,
     where reading the weight is the cost: up to 64 rows read it once, more rows once per 64.

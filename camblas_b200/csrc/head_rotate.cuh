@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
 
 template <int Lanes, int Batch> void launch_batch(camblas_cuda_context *context, const RotateTask &task, int parts)
 {
-    const dim3 grid(task.tokens, parts);
+    const dim3 grid(task.tokens, parts < 65535 ? parts : 65535); /* the kernel goes round for more */
     if (task.interleaved)
         rotate_kernel<Lanes, Batch, true><<<grid, kThreads, 0, context->stream>>>(task);
     else

@@ -26,9 +26,10 @@
  *   sum (c - z) x = sum c x - z sum x.
  *
  * The tokens are brought to FP16 first, in a small kernel of their own:
- * spread_tokens divides each 128 inputs of a token by a power of two that brings
- * the largest to [1, 2) (an FP16 then holds a BF16 exactly down to 2^-21 of that
- * and below it to within 2^-25 of the largest), and leaves the power and the sum
+ * spread_tokens multiplies each 128 inputs of a token by a power of two that
+ * brings the largest to [2^14, 2^15), where an FP16 holds a BF16 exactly down to
+ * 2^-31 of the largest (its least step is 2^-24, a BF16's 2^-7 of its own power of
+ * two) and below that to within 2^-39 of it, and leaves the power and the sum
  * of every group. linear_kernel is its programmatic dependent and has its
  * first weights in flight before it waits for the tokens. A token element that
  * is infinite or NaN makes the token's outputs NaN.
@@ -105,9 +106,7 @@ template <int Group> __global__ void __launch_bounds__(256) spread_tokens(const 
 #pragma unroll
     for (int offset = 1; offset < 16; offset *= 2)
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
-    int exponent = 0; /* of zero and of what is not finite: 0 */
-    if (largest > 0.f && largest < INFINITY)
-        exponent = max(-126, min(126, (__float_as_int(largest) >> 23) - 127));
+    const int exponent = attend::half_exponent(largest);
     const float down = __int_as_float((127 - exponent) << 23), up = __int_as_float((127 + exponent) << 23);
     uint4 halves;
     halves.x = attend::pack<true>(low.e[0] * down, low.e[1] * down);
@@ -152,6 +151,10 @@ __device__ __forceinline__ float2 scale_pair(const __nv_bfloat16 *from)
 {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(from));
 }
+
+/* The scales of outputs g and g + 8 with the factors of their codes taken back, before a token's power
+ * comes in: a small power times 2^-24 would leave FP32's normal numbers. */
+__device__ __forceinline__ float2 raised(float2 scales) { return make_float2(scales.x * 0x1p24f, scales.y * 0x1p20f); }
 
 /* Zero points of outputs g and g + 8, the second times 16 like its codes; a byte in the low bits of
  * 2^23 is that number. */
@@ -329,7 +332,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
                 uint4 words;
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i) {
-                    const float2 s = scale_pair(reinterpret_cast<const Scale *>(own + S::kScalesAt) + 16 * i + 2 * g);
+                    const float2 s =
+                        raised(scale_pair(reinterpret_cast<const Scale *>(own + S::kScalesAt) + 16 * i + 2 * g));
                     float2 z = make_float2(8.f, 128.f);
                     if constexpr (Zeros)
                         z = zero_pair(*reinterpret_cast<const uint16_t *>(own + S::kZerosAt + 16 * i + 2 * g));
@@ -382,8 +386,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
 #pragma unroll
         for (int n = 0; n < Columns; ++n) {
             float *to = exchange + (8 * n + 2 * t) * S::kPitch + warp * 16 + g;
-            to[0] = sum[n][0] * 0x1p24f, to[S::kPitch] = sum[n][1] * 0x1p24f;
-            to[8] = sum[n][2] * 0x1p20f, to[S::kPitch + 8] = sum[n][3] * 0x1p20f;
+            to[0] = sum[n][0], to[S::kPitch] = sum[n][1];
+            to[8] = sum[n][2], to[S::kPitch + 8] = sum[n][3];
         }
     }
     if (task.split > 1)
@@ -512,11 +516,11 @@ __global__ void __launch_bounds__(kWarps * 32, 7) few_kernel(const __grid_consta
                 float2 z = make_float2(8.f, 128.f);
                 if constexpr (Zeros)
                     z = zero_pair(held[d].zeros[i]);
-                const float s0 = float(held[d].scales[i].low), s1 = float(held[d].scales[i].high);
-                low.x = fmaf(s0, fmaf(-z.x, taken.x, part_sum[0][0]), low.x);
-                low.y = fmaf(s0, fmaf(-z.x, taken.y, part_sum[0][1]), low.y);
-                high.x = fmaf(s1, fmaf(-z.y, taken.x, part_sum[0][2]), high.x);
-                high.y = fmaf(s1, fmaf(-z.y, taken.y, part_sum[0][3]), high.y);
+                const float2 s = raised(make_float2(float(held[d].scales[i].low), float(held[d].scales[i].high)));
+                low.x = fmaf(s.x, fmaf(-z.x, taken.x, part_sum[0][0]), low.x);
+                low.y = fmaf(s.x, fmaf(-z.x, taken.y, part_sum[0][1]), low.y);
+                high.x = fmaf(s.y, fmaf(-z.y, taken.x, part_sum[0][2]), high.x);
+                high.y = fmaf(s.y, fmaf(-z.y, taken.y, part_sum[0][3]), high.y);
             }
             fetch(held[d], base + d + kAhead);
             sum[0] = fmaf(power.x, low.x, sum[0]), sum[1] = fmaf(power.y, low.y, sum[1]);
@@ -524,8 +528,8 @@ __global__ void __launch_bounds__(kWarps * 32, 7) few_kernel(const __grid_consta
             unit_tokens += pitch;
         }
     }
-    exchange[warp][2 * t][g] = sum[0] * 0x1p24f, exchange[warp][2 * t + 1][g] = sum[1] * 0x1p24f;
-    exchange[warp][2 * t][g + 8] = sum[2] * 0x1p20f, exchange[warp][2 * t + 1][g + 8] = sum[3] * 0x1p20f;
+    exchange[warp][2 * t][g] = sum[0], exchange[warp][2 * t + 1][g] = sum[1];
+    exchange[warp][2 * t][g + 8] = sum[2], exchange[warp][2 * t + 1][g + 8] = sum[3];
     if (task.split > 1)
         cluster_barrier();
     else

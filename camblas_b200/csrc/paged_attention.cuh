@@ -289,6 +289,16 @@ __device__ __forceinline__ float power_of_two(float x)
     return y;
 }
 
+/* The exponent of the power of two that is divided out of BF16 numbers, the largest of which is
+ * `largest`, to bring that to [2^14, 2^15), the top of FP16's range; 0 for zero and for what is not
+ * finite. Both 2^exponent and 2^-exponent are normal numbers. */
+__device__ __forceinline__ int half_exponent(float largest)
+{
+    if (!(largest > 0.f && largest < INFINITY))
+        return 0;
+    return max(-126, (__float_as_int(largest) >> 23) - 127 - 14);
+}
+
 /* two E4M3 values (exact in FP16), the lower byte in the lower half */
 __device__ __forceinline__ uint32_t widen(uint32_t two_bytes)
 {
@@ -490,8 +500,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
                         }
                     head_scale[n][0] = head_scale[n][1] = task.score_scale;
                 } else {
-                    /* To FP16, whose mantissa holds a BF16 but whose range does not: divided by
-                     * a power of two that brings the head's largest element to [1, 2). */
+                    /* To FP16, whose mantissa holds a BF16 but whose range does not: divided by a
+                     * power of two of the head's largest element. */
                     uint2 raw[S::kPieces];
                     float largest = 0.f;
 #pragma unroll
@@ -506,9 +516,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
                     }
                     largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
                     largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                    int exponent = 0; /* of zero and of what is not finite: 0 */
-                    if (largest > 0.f && largest < INFINITY)
-                        exponent = max(-126, min(126, (__float_as_int(largest) >> 23) - 127));
+                    const int exponent = half_exponent(largest);
                     const float down = __int_as_float((127 - exponent) << 23);
                     const float up = __int_as_float((127 + exponent) << 23);
 #pragma unroll

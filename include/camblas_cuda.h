@@ -533,8 +533,8 @@ int camblas_cuda_paged_attention(camblas_cuda_context *context, int batch, int h
  * inner] . W^T (+ bias) (+ residual), BF16, where W[o,k] = (code - zero) *
  * scale, code and zero whole numbers 0..15 (zero 8 when zeros is NULL), scale
  * and zero of output o and group k / group. Products of exact operands, FP32
- * sums, scales applied in FP32, one rounding (of x, what lies below 2^-21 of the
- * largest of its 128 inputs keeps an absolute error of 2^-25 of that; an element
+ * sums, scales applied in FP32, one rounding (of x, what lies below 2^-31 of the
+ * largest of its 128 inputs keeps an absolute error of 2^-39 of that; an element
  * that is not finite makes its token's outputs NaN). scale_type 0 FP32, 2 BF16;
  * zeros 1 when the weights hold zero points. weights is what the Int4Weight class
  * of the Python layer produces: [blocks of 64 outputs][units of 128 inputs][4

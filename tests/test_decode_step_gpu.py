@@ -170,6 +170,8 @@ def paged(gen, lengths, page, kv_heads, depth, kind=BF16, spare=3):
     (9, 9, 80, 8, (65, 1, 0, 12), 5, 2),
     (4, 2, 16, 2, (40,), 39, 7),
     (2, 2, 208, 1, (90, 91), 1, 0),
+    (3, 3, 72, 16, (33, 0, 70), 0, 0),
+    (5, 1, 8, 4, (100,), 30, 2),
 ])
 def test_paged_attention(gen, kind, heads, kv_heads, depth, page, lengths, window, sinks):
     if kind == E4M3 and depth % 16:
@@ -364,6 +366,24 @@ def test_int4_linear(gen, rows, outputs, inner, group, zeros, scale_type):
     extra = bound + 2 * exact.U32 * (want.abs() + bias.double().abs() + residual.double().abs())
     assert exact.within(_kernels.int4_linear(x, weight, bias, residual),
                         want + bias.double() + residual.double(), extra)
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_int4_tokens_of_any_size(gen, rows):
+    """Powers of two far beyond FP16's range and spread within a token keep the result's accuracy; what is not
+    finite stays in its own token."""
+    codes, scale, zero = int4_case(gen, 70, 256, 64, True)
+    weight = _kernels.Int4Weight(codes, scale, zero)
+    x = normal(gen, rows, 256).to(BF16)
+    x[0] *= 2.0 ** 100
+    x[1] *= 2.0 ** -120
+    x[2, ::3] *= 2.0 ** -25
+    want, bound = exact.int4(x, codes, scale, zero)
+    assert exact.within(_kernels.int4_linear(x, weight), want, bound)
+    clean = _kernels.int4_linear(x, weight)
+    x[0, 17], x[1, 200] = float("inf"), float("nan")
+    out = _kernels.int4_linear(x, weight)
+    assert out[:2].isnan().all() and torch.equal(out[2:], clean[2:])
 
 
 def test_int4_picks_single_weights(gen):
