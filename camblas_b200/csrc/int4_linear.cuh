@@ -21,7 +21,8 @@
  * n * 2^-24, exact, and in the next four bits 16 n * 2^-24; so a pair of codes is
  * one AND of the word, or of the word shifted by 8, and five instructions unpack
  * a product's operand. (128 + n in BF16, less 128 + z, takes eleven, and then
- * issue and not HBM is the bound.) The factors 2^24 and 1/16 go to the scales,
+ * issue and not HBM is the bound: 70 us for one token, 28672 -> 8192, where this
+ * takes 30.) The factors 2^24 and 1/16 go to the scales,
  * and the zero point is taken out of the group's sum in FP32:
  *   sum (c - z) x = sum c x - z sum x.
  *
@@ -30,8 +31,8 @@
  * brings the largest to [2^14, 2^15), where an FP16 holds a BF16 exactly down to
  * 2^-31 of the largest (its least step is 2^-24, a BF16's 2^-7 of its own power of
  * two) and below that to within 2^-39 of it, and leaves the power and the sum
- * of every group. linear_kernel is its programmatic dependent and has its
- * first weights in flight before it waits for the tokens. A token element that
+ * of every group. The product is its programmatic dependent and has its first
+ * weights in flight before it waits for the tokens. A token element that
  * is infinite or NaN makes the token's outputs NaN.
  *
  * Layout: [block of 64 outputs][unit of 128 inputs][4 tiles of 16 outputs], a
@@ -210,7 +211,7 @@ template <int Columns, int Group, typename Scale, bool Zeros> struct Stage {
      * 64), and the rows of two tokens apart start eight banks apart for the stores. */
     static constexpr int kPitch = kWarps * 16 + 4;
     static constexpr int kExchange = kTokens * kPitch * 4;
-    static constexpr int kFitRegisters = Columns > 2 ? 3 : 5; /* CTAs on an SM */
+    static constexpr int kFitRegisters = Columns > 2 ? 3 : (Columns > 1 ? 5 : 7); /* CTAs on an SM */
 
     static __host__ __device__ constexpr int pass_bytes(int live) { return kFactorBytes + live * kTokenBytes; }
     static __host__ __device__ constexpr int bytes(int live) { return kTokensAt + kUnits * pass_bytes(live); }
@@ -564,8 +565,9 @@ __global__ void __launch_bounds__(kWarps * 32, 7) few_kernel(const __grid_consta
 /* Ranges of the units per block of outputs (the ranks of a cluster), by a rough
  * model of the time: a CTA alone on an SM takes `alone` for a unit, k CTAs
  * together `shared` each (what HBM gives an SM, or the products of the columns),
- * and CTAs that do not fit wait. Measured on one token, 28672 -> 8192: one range
- * 84 us, eight 24 us. */
+ * and CTAs that do not fit wait. Measured (37 tokens, 7168 -> 4992, groups of
+ * 128): 23.6, 22.8, 23.1, 23.6 and 23.2 us with 1, 2, 3, 4 and 7 ranges, the
+ * chosen one 22.2; 64 outputs alone would leave 147 SMs without work. */
 inline int choose_split(int blocks, int units, int step, int columns, int sm_count, int resident)
 {
     const double alone = 0.15 + 0.06 * columns, shared = 0.05 * columns > 0.1 ? 0.05 * columns : 0.1;
@@ -670,7 +672,7 @@ template <int Columns, int Group, typename Scale> int allow_shared()
 
 template <int Group, typename Scale> int allow_shared_group()
 {
-    return allow_shared<2, Group, Scale>() | allow_shared<4, Group, Scale>() |
+    return allow_shared<1, Group, Scale>() | allow_shared<2, Group, Scale>() | allow_shared<4, Group, Scale>() |
            allow_shared<6, Group, Scale>() | allow_shared<8, Group, Scale>();
 }
 
@@ -685,8 +687,12 @@ inline int prepare_kernels()
 template <int Group, typename Scale>
 cudaError_t launch_rows(camblas_cuda_context *context, const LinearTask &task, bool zeros)
 {
-    if (task.pass_rows == 8)
-        return launch_few<Group, Scale>(context, task, zeros);
+    /* few_kernel while one wave of its CTAs has a place for every tile of outputs; with more, the
+     * block kernel keeps its ring full where few_kernel would start anew (one token, 8192 -> 28672:
+     * 50 us by few_kernel, 40 by the block kernel; 28672 -> 8192: 30 and 42) */
+    if (task.rows <= 8)
+        return (task.outputs + 15) / 16 <= 7ll * context->sm_count ? launch_few<Group, Scale>(context, task, zeros)
+                                                                   : launch<1, Group, Scale>(context, task, zeros);
     if (task.rows <= 16)
         return launch<2, Group, Scale>(context, task, zeros);
     if (task.rows <= 32)
@@ -717,20 +723,15 @@ inline bool sizes_bad(int rows, int inner, int group)
            (group != 32 && group != 64 && group != 128) || inner % group;
 }
 
-/* Tokens of a pass: all of them where that goes. Eight mean few_kernel, which is
- * taken while one wave of its CTAs has a place for every tile of outputs; with
- * more outputs (one token, 8192 -> 28672: 50 us) the block kernel keeps its ring
- * full from tile to tile (46 us). */
-inline int rows_of_pass(int rows, int outputs, int sm_count)
+/* Tokens of a pass: all of them where that goes. */
+inline int rows_of_pass(int rows)
 {
-    if (rows <= 8 && (outputs + 15) / 16 <= 7ll * sm_count)
-        return 8;
-    return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 48 ? 48 : 64));
+    return rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 48 ? 48 : 64)));
 }
 
 inline size_t workspace_bytes(int rows, int inner, int group)
 {
-    const size_t units = (inner + kUnit - 1) / kUnit, pass_rows = rows_of_pass(rows, INT_MAX, 1);
+    const size_t units = (inner + kUnit - 1) / kUnit, pass_rows = rows_of_pass(rows);
     const size_t passes = (rows + pass_rows - 1) / pass_rows;
     return units * (passes * factor_bytes(group, int(pass_rows)) + size_t(rows) * kTokenBytes);
 }
@@ -767,7 +768,7 @@ extern "C" int camblas_cuda_int4_linear(camblas_cuda_context *context, int rows,
             return host::fail(context, "4-bit linear workspace too small", 1);
         nibble::LinearTask task{};
         task.rows = rows, task.inner = inner, task.outputs = outputs;
-        task.units = (inner + nibble::kUnit - 1) / nibble::kUnit, task.pass_rows = nibble::rows_of_pass(rows, outputs, context->sm_count);
+        task.units = (inner + nibble::kUnit - 1) / nibble::kUnit, task.pass_rows = nibble::rows_of_pass(rows);
         task.x = static_cast<const __nv_bfloat16 *>(x), task.ldx = ldx;
         task.weights = static_cast<const uint8_t *>(weights);
         task.bias = static_cast<const __nv_bfloat16 *>(bias);

@@ -11,16 +11,23 @@
  * Bound: every visible key and value has to be read once, 2 * depth values per
  * token and key head, for 4 * depth * (heads / kv_heads) operations, so HBM
  * bounds it for any group of heads that one pass serves; the products go to the
- * tensor cores because eight heads per key on CUDA cores would not keep up. The work of a warp is 16
- * tokens: S^T[16 tokens, 8 heads] = K Q^T and O^T[depth, 8 heads] += V^T P^T
- * with mma.m16n8k16. Tokens (and depth) take the 16-row side, so that a group
- * of up to eight heads fills the 8-column side, and the softmax statistics of a
- * head sit on the lanes that hold the head's column in both products. P^T turns
- * from the accumulator's to the operand's layout by movmatrix, without shared
- * memory. (tcgen05 would want 128 rows of M and bring nothing to a kernel that
- * waits for HBM.) Scores, statistics, sums and the joined result are FP32; P is
- * rounded to BF16 (to FP16 over an 8-bit cache), at most half a step relative
- * to each weight, like the operands of any BF16 product.
+ * tensor cores because eight heads per key on CUDA cores would not keep up. A
+ * warp's tile is 16, 32 or 64 tokens, 8 KB (16 KB at 256 BF16 columns): S^T[16
+ * tokens, 8 heads] = K Q^T and O^T[depth, 8 heads] += V^T P^T with mma.m16n8k16.
+ * Tokens (and depth) take the 16-row side, so that a group of up to eight heads
+ * fills the 8-column side, and the softmax statistics of a head sit on the lanes
+ * that hold the head's column in both products. P^T turns from the accumulator's
+ * to the operand's layout by movmatrix, without shared memory. (tcgen05 would
+ * want 128 rows of M and bring nothing to a kernel that waits for HBM; mma.sync
+ * does a product in 8 cycles per sub-core here, a quarter of the time that HBM
+ * gives.) Scores, statistics, sums and the joined result are FP32; P is rounded to
+ * BF16 (to FP16 over an 8-bit cache), at most half a step relative to each weight,
+ * like the operands of any BF16 product.
+ *
+ * Measured, 64 query and 8 key heads of 128 in BF16: one sequence of 130977
+ * tokens 98 us (0.84 of the measured copy rate), 48 sequences of 0 to 8191 tokens
+ * 60 us (0.61; some 5 us are the way from the lengths to the first keys, and 11
+ * the join), one of 300 tokens 10.7 us.
  *
  * Work split. A warp works alone. The slots of a sequence (key heads times
  * blocks of 8 or 16 query heads) are taken in teams of four neighbours, two or
