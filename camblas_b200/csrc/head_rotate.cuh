@@ -72,11 +72,6 @@ __device__ __forceinline__ Piece unpack_piece(const uint2 &raw)
     return {{low.x, low.y, high.x, high.y}};
 }
 
-__device__ __forceinline__ Piece load_piece(const __nv_bfloat16 *from)
-{
-    return unpack_piece(*reinterpret_cast<const uint2 *>(from));
-}
-
 __device__ __forceinline__ void store_piece(__nv_bfloat16 *to, const Piece &p)
 {
     const __nv_bfloat162 low = __floats2bfloat162_rn(p.e[0], p.e[1]);

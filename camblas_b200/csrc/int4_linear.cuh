@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
     for (int n = 0; n < Columns; ++n)
         sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
 
+    int issued = 0; /* stages, by the producing thread */
     if (warp == kWarps) {
         if (lane == 0) {
             const uint8_t *weights = task.weights + (long long)block * task.units * (kWarps * S::kTileBytes);
@@ -297,6 +298,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
             asm volatile("griddepcontrol.wait;" ::: "memory");
             for (int step = 0; step < ahead; ++step)
                 load_tokens(step);
+            issued = ahead;
             for (int step = ahead; step < steps; ++step) {
                 if (!sm100::mbar_wait(&empty[step % kStages], (step / kStages - 1) & 1, abort)) {
                     sm100::report(task.status, abort, sm100::kRoleProducer);
@@ -304,6 +306,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
                 }
                 load_weights(step);
                 load_tokens(step);
+                ++issued;
             }
         }
         __syncwarp();
@@ -382,6 +385,11 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
      * order, for its share of the outputs. */
     __syncthreads();
     const bool ok = *abort == 0;
+    if (!ok && threadIdx.x == kWarps * 32) { /* a wait gave up: the copies under way get as long again */
+        volatile uint32_t never = 0;
+        for (int step = max(0, issued - kStages); step < issued; ++step)
+            sm100::mbar_wait(&full[step % kStages], (step / kStages) & 1, &never);
+    }
     float *exchange = reinterpret_cast<float *>(shared);
     if (ok && warp < kWarps) {
 #pragma unroll

@@ -283,6 +283,16 @@ def test_many_sequences_of_all_lengths(gen):
     assert exact.within(out, want, bound)
 
 
+def test_a_large_batch_of_short_sequences(gen):
+    """Several scans of 32 lengths, three key heads (one warp per team), sequences without tokens at both ends."""
+    lengths = [0] + [int(v) for v in integers(gen, 0, 40, 698)] + [0]
+    keys, values, table, counts = paged(gen, lengths, 8, 3, 32)
+    q = normal(gen, 700, 3, 32).to(BF16)
+    out = _kernels.paged_attention(q, keys, values, table, counts)
+    want, bound = exact.attention(q, keys, values, table, counts, 32 ** -0.5, 0, 0)
+    assert exact.within(out, want, bound)
+
+
 def test_attention_in_graphs_follows_lengths(gen):
     """Two graphs of the same call on two streams, replayed side by side, with lengths that changed since."""
     keys, values, table, counts = paged(gen, (600, 600), 16, 2, 128)
@@ -509,6 +519,15 @@ def test_closed_and_broken_rows(gen):
     ids, weights = _kernels.route_experts(logits, 4, scoring="sigmoid")
     assert 7 not in ids[3].tolist() and weights[3].isfinite().all()
     assert ids[4, 0] == 5
+
+
+def test_more_tokens_than_a_grid_holds(gen):
+    logits = normal(gen, 270001, 12)
+    ids, weights = _kernels.route_experts(logits, 3, scoring="sigmoid", renormalise=False)
+    ranked = logits.double().sort(dim=1, descending=True, stable=True)
+    assert torch.equal(ids, ranked.indices[:, :3])
+    want = torch.sigmoid(ranked.values[:, :3])
+    assert ((weights.double() - want).abs() <= (exact.U32 * 1.001 + 1e-12) * want).all()
 
 
 def test_route_strided_and_refusals(gen):
