@@ -172,6 +172,9 @@ def paged(gen, lengths, page, kv_heads, depth, kind=BF16, spare=3):
     (2, 2, 208, 1, (90, 91), 1, 0),
     (3, 3, 72, 16, (33, 0, 70), 0, 0),
     (5, 1, 8, 4, (100,), 30, 2),
+    (256, 1, 64, 1000, (400, 77), 0, 0),
+    (33, 1, 128, 16, (260, 5), 0, 0),
+    (36, 2, 192, 128, (150,), 2 ** 31 - 1, 2 ** 31 - 1),
 ])
 def test_paged_attention(gen, kind, heads, kv_heads, depth, page, lengths, window, sinks):
     if kind == E4M3 and depth % 16:
@@ -422,6 +425,29 @@ def test_int4_strided_and_shaped_operands(gen):
     assert torch.equal(_kernels.int4_linear(wide[:, 8:264], weight, residual=residual[:, 4:100]),
                        _kernels.int4_linear(wide[:, 8:264], weight, residual=residual[:, 4:100].contiguous()))
     assert _kernels.int4_linear(wide[:0, 8:264], weight).shape == (0, 96)
+
+
+@pytest.mark.parametrize("rows", [2, 20])
+def test_int4_captured_beside_another_call(gen, rows):
+    """A captured product keeps its own workspace: replays beside eager calls of other tokens give its own result."""
+    codes, scale, zero = int4_case(gen, 300, 1024, 64, True)
+    weight = _kernels.Int4Weight(codes, scale, zero)
+    x, other = normal(gen, rows, 1024).to(BF16), normal(gen, rows, 1024).to(BF16)
+    expected = [_kernels.int4_linear(value, weight) for value in (x, other)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        _kernels.int4_linear(x, weight)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = _kernels.int4_linear(x, weight)
+    for _ in range(20):
+        with torch.cuda.stream(stream):
+            graph.replay()
+        assert torch.equal(_kernels.int4_linear(other, weight), expected[1])
+        stream.synchronize()
+        assert torch.equal(out, expected[0])
 
 
 def test_int4_leaves_its_neighbours_alone(gen):
