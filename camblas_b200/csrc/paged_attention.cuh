@@ -27,7 +27,7 @@
  * Measured, 64 query and 8 key heads of 128 in BF16: one sequence of 130977
  * tokens 98 us (0.84 of the measured copy rate), 48 sequences of 0 to 8191 tokens
  * 60 us (0.61; some 5 us are the way from the lengths to the first keys, and 11
- * the join), one of 300 tokens 10.7 us.
+ * the join), one of 300 tokens 9.5 us.
  *
  * Work split. A warp works alone. The slots of a sequence (key heads times
  * blocks of 8 or 16 query heads) are taken in teams of four neighbours, two or
@@ -335,9 +335,12 @@ template <int Depth, int Blocks, bool Eight> struct Shape {
     static constexpr int kGroups = kTile / 16; /* of 16 tokens */
     static constexpr int kTileShift = kTile == 16 ? 4 : (kTile == 32 ? 5 : 6);
     static constexpr int kTileBytes = 2 * kTile * kRowBytes; /* keys and values */
-    /* The copies in flight on an SM have to cover the latency of HBM at its share of the
-     * bandwidth, some 45 KB. */
-    static constexpr int kStages = kRowBytes >= 512 ? 3 : 2;
+    /* The copies in flight on an SM have to cover the latency of HBM at its share of the bandwidth,
+     * some 45 KB. Two stages do, and let more warps share the SM (48 ragged sequences of 128 BF16
+     * columns: 60 us, three stages 65), unless registers keep the third CTA away or make it spill:
+     * sixteen heads at 128 BF16 columns (eight sequences, one key head: 28 us with three, 34 with
+     * two). */
+    static constexpr int kStages = kRowBytes >= 512 || (kRowBytes == 256 && Blocks == 2) ? 3 : 2;
     static constexpr int kNoteBytes = 16 * kTile + 16; /* where the rows of a stage lie, which are real */
     static constexpr int kWarpBytes = kStages * (kTileBytes + kNoteBytes);
     static constexpr int kBytes = kWarps * kWarpBytes;
@@ -933,7 +936,8 @@ cudaError_t launch_join(camblas_cuda_context *context, const AttendTask &task, c
     const int expected = plan.grid * kWarps / items + 2;
     if (expected > 32)
         return launch_join_of<Eight, 1, 8>(context, task, plan, 16);
-    return launch_join_of<Eight, 2, 4>(context, task, plan, expected > 16 ? 4 : (expected > 4 ? 2 : 1));
+    return launch_join_of<Eight, 2, 4>(context, task, plan,
+                                       expected > 16 ? 8 : (expected > 8 ? 4 : (expected > 4 ? 2 : 1)));
 }
 
 template <int Depth, int Blocks, bool Eight> int allow_shared(Shape<Depth, Blocks, Eight>)
