@@ -20,13 +20,14 @@
  * to the operand's layout by movmatrix, without shared memory. (tcgen05 would
  * want 128 rows of M and bring nothing to a kernel that waits for HBM; mma.sync
  * does a product in 8 cycles per sub-core here, a quarter of the time that HBM
- * gives.) Scores, statistics, sums and the joined result are FP32; P is rounded to
- * BF16 (to FP16 over an 8-bit cache), at most half a step relative to each weight,
- * like the operands of any BF16 product. FP16 keeps that only down to 2^-14, and a
- * result can be made of weights far below the largest (a first token that takes the
- * weight and has next to no value), so over an 8-bit cache P is 2^15 times the
- * weights: those down to 2^-29 of the largest are rounded by half a step, those
- * below to within 2^-40 of it.
+ * gives.) Scores, statistics, sums and the joined result are FP32; P goes to the
+ * value product in two parts, rounded to BF16 and what that leaves, rounded again
+ * (over an 8-bit cache FP16): at most 2^-16 (2^-22) of each weight is lost. In one
+ * part the 2^-8 (2^-11) of each weight made the result's error against 64 bits 3 to
+ * 13 % larger than its last rounding alone. FP16 keeps its bits only down to 2^-14,
+ * and a result can be made of weights far below the largest (a first token that
+ * takes the weight and has next to no value), so over an 8-bit cache P is 2^15 times
+ * the weights, and what lies below 2^-40 of the largest is lost.
  *
  * Measured, 64 query and 8 key heads of 128 in BF16: one sequence of 130977
  * tokens 98 us (0.84 of the measured copy rate), 48 sequences of 0 to 8191 tokens
@@ -291,6 +292,14 @@ template <bool Half> __device__ __forceinline__ uint32_t pack(float low, float h
         const __nv_bfloat162 pair = __floats2bfloat162_rn(low, high);
         return *reinterpret_cast<const uint32_t *>(&pair);
     }
+}
+
+template <bool Half> __device__ __forceinline__ float2 unpack(uint32_t raw)
+{
+    if constexpr (Half)
+        return __half22float2(*reinterpret_cast<const __half2 *>(&raw));
+    else
+        return make_float2(__uint_as_float(raw << 16), __uint_as_float(raw & 0xffff0000u));
 }
 
 /* 2^x; 0 for -infinity */
@@ -598,7 +607,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
                     for (int n = 0; n < Blocks; ++n)
                         mma_16816<Eight>(s[n][m][kk % kChains], a, qf[n][kk][0], qf[n][kk][1]);
                 }
-            uint32_t p[Blocks][S::kGroups][2];
+            uint32_t p[Blocks][S::kGroups][2], rest[Blocks][S::kGroups][2];
             bool rescale = false;
             float factor[Blocks][2];
 #pragma unroll
@@ -636,8 +645,14 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
                         sum[n][i & 1] += score[m][i];
                     }
                     constexpr float kFactor = Eight ? kRaised : 1.f;
-                    p[n][m][0] = transpose_8x8(pack<Eight>(score[m][0] * kFactor, score[m][1] * kFactor));
-                    p[n][m][1] = transpose_8x8(pack<Eight>(score[m][2] * kFactor, score[m][3] * kFactor));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float low = score[m][2 * i] * kFactor, high = score[m][2 * i + 1] * kFactor;
+                        const uint32_t rounded = pack<Eight>(low, high);
+                        const float2 taken = unpack<Eight>(rounded);
+                        p[n][m][i] = transpose_8x8(rounded);
+                        rest[n][m][i] = transpose_8x8(pack<Eight>(low - taken.x, high - taken.y));
+                    }
                 }
             }
             if (__any_sync(0xffffffffu, rescale)) {
@@ -658,8 +673,10 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
                         const int row = 16 * m + (lane & 7) + (lane / 16) * 8, part = 2 * j + ((lane / 8) & 1);
                         ldmatrix_x4_trans(a, values + row * S::kRowBytes + S::place(row, part));
 #pragma unroll
-                        for (int n = 0; n < Blocks; ++n)
+                        for (int n = 0; n < Blocks; ++n) {
                             mma_16816<false>(o[n][j], a, p[n][m][0], p[n][m][1]);
+                            mma_16816<false>(o[n][j], a, rest[n][m][0], rest[n][m][1]);
+                        }
                     }
                 } else {
                     /* lane (g, t): depths 32 J + 4g + i, i = 0..3, of tokens 2t, 2t+1, 2t+8, 2t+9:
@@ -686,6 +703,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
                         for (int n = 0; n < Blocks; ++n) {
                             mma_16816<true>(o[n][2 * J], even, p[n][m][0], p[n][m][1]);
                             mma_16816<true>(o[n][2 * J + 1], odd, p[n][m][0], p[n][m][1]);
+                            mma_16816<true>(o[n][2 * J], even, rest[n][m][0], rest[n][m][1]);
+                            mma_16816<true>(o[n][2 * J + 1], odd, rest[n][m][0], rest[n][m][1]);
                         }
                     }
                 }

@@ -39,3 +39,26 @@ def test_small_weights_beside_a_dominant_token(gen, kind, heads, depth, ahead):
     out = _kernels.paged_attention(q, keys, values, table, counts, scale=ahead / 64)
     want, bound = exact.attention(q, keys, values, table, counts, ahead / 64, 0, 0)
     assert exact.within(out, want, bound)
+
+
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+@pytest.mark.parametrize("heads,depth,length", [(1, 64, 23), (8, 128, 64), (16, 128, 40), (2, 256, 17), (12, 16, 61)])
+def test_weights_keep_more_bits_than_the_values(gen, kind, heads, depth, length):
+    """Values that nearly cancel under the weights show the rounding of the weights, which the result's own
+    rounding hides elsewhere: two parts of eight (eleven) bits leave at most 2^-16 (2^-22) of each."""
+    keys, values, table, counts = paged(gen, (length,), 16, 1, depth, kind)
+    q = (0.5 * normal(gen, 1, heads, depth)).to(BF16)
+    scale = depth ** -0.5
+    last = int(table[0, (length - 1) // 16]), (length - 1) % 16
+    k = torch.stack([keys[int(table[0, t // 16]), t % 16, 0] for t in range(length)]).double()
+    v = torch.stack([values[int(table[0, t // 16]), t % 16, 0] for t in range(length)]).double()
+    p = torch.softmax(scale * (q[0].double() @ k.t()), -1)[0]  # of the first head
+    values[last][0] = (-(p[:-1] @ v[:-1]) / p[-1]).clamp(-400, 400).to(kind)
+    out = _kernels.paged_attention(q, keys, values, table, counts, scale=scale)
+    want, bound = exact.attention(q, keys, values, table, counts, scale, 0, 0)
+    # the oracle's bound holds one rounding of the weights to BF16 (FP16); in its place the second part's
+    half = exact.HALF_STEP[BF16 if kind is BF16 else torch.float16]
+    v[-1] = values[last][0].double()
+    p = torch.softmax(scale * (q[0].double() @ k.t()), -1)
+    bound = bound - (half - half * half) * (p @ v.abs())[None]
+    assert exact.within(out, want, bound)
