@@ -1027,7 +1027,7 @@ extern "C" int camblas_cuda_paged_attention(
         bool bad = !q || !strides || !lengths || !output ||
                    (table_width > 0 && !table) || (pages > 0 && (!key_cache || !value_cache));
         bad = bad || heads::misaligned(q, 8) || heads::misaligned(table, 4) || heads::misaligned(lengths, 4) ||
-              heads::misaligned(output, 2) || q == output || key_cache == output || value_cache == output;
+              heads::misaligned(output, 4) /* stored in pairs */ || q == output || key_cache == output || value_cache == output;
         if (!bad) {
             task.keys = {const_cast<void *>(key_cache), strides[2], strides[3], strides[4]};
             task.values = {const_cast<void *>(value_cache), strides[5], strides[6], strides[7]};

@@ -62,3 +62,29 @@ def test_weights_keep_more_bits_than_the_values(gen, kind, heads, depth, length)
     p = torch.softmax(scale * (q[0].double() @ k.t()), -1)
     bound = bound - (half - half * half) * (p @ v.abs())[None]
     assert exact.within(out, want, bound)
+
+
+def attention_by_c(gen, batch=2, offset=0):
+    """Status, message and output of a small call through the C ABI, the output `offset` elements into its buffer."""
+    keys, values, table, counts = paged(gen, (30, 20), 16, 2, 64)
+    q = normal(gen, 2, 4, 64).to(BF16)
+    strides = (ct.c_longlong * 9)(q.stride(0), q.stride(1), *keys.stride()[:3], *values.stride()[:3], table.stride(0))
+    size = _native.context(0).workspace_bytes("paged_attention", 2, 4, 2, 64, 2, 16, table.shape[1], 0, 0)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    buffer = torch.zeros(q.numel() + 4, dtype=BF16, device="cuda")
+    out = buffer[offset:offset + q.numel()].view(q.shape)
+    status, context = raw("paged_attention", batch, 4, 2, 64, 0.125, pointer(q), 2, pointer(keys), pointer(values),
+                          strides, keys.shape[0], 16, 1.0, 1.0, pointer(table), table.shape[1], pointer(counts), 0, 0,
+                          pointer(workspace), size, pointer(out))
+    if status:
+        assert not buffer.any()
+    else:
+        assert torch.equal(out, _kernels.paged_attention(q, keys, values, table, counts))
+    return status, error_text(context) if status else ""
+
+
+def test_attention_refuses_an_output_off_its_pairs(gen):
+    for offset in (1, 3):
+        status, message = attention_by_c(gen, offset=offset)
+        assert status < 0 and "operands" in message
+    assert attention_by_c(gen)[0] == 0 and attention_by_c(gen, offset=2)[0] == 0
