@@ -915,7 +915,7 @@ def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, windo
     kv_heads = key_cache.shape[2] if key_cache.dim() == 4 else 0
     code, pages, page_size, strides = _check_caches(key_cache, value_cache, index, kv_heads, depth,
                                                     8 if key_cache.dtype is torch.bfloat16 else 16)
-    if (kv_heads < 1 or not 1 <= heads <= 65536 or heads % kv_heads or batch * heads > _INT_MAX
+    if (kv_heads < 1 or not 1 <= heads <= 65536 or heads % kv_heads or batch * heads > _INT_MAX - 63
             or not 8 <= depth <= 256 or depth & (15 if code == 3 else 7)):
         raise ValueError("paged_attention takes heads a multiple of kv_heads and a depth of a multiple of 8 "
                          "(E4M3: 16) up to 256")

@@ -984,13 +984,16 @@ inline int prepare_kernels()
     return status;
 }
 
+/* Query heads of a call: the scans of the lengths count up to the next multiple of 32, in 32 bits. */
+constexpr int kMostHeads = INT_MAX - 63;
+
 inline bool sizes_bad(int batch, int heads_count, int kv_heads, int depth, int cache_type, int page_size,
                       int table_width, int window, int sinks)
 {
     return batch < 0 || kv_heads < 1 || heads_count < 1 || heads_count > 65536 || heads_count % kv_heads ||
            depth < 8 || depth > 256 || (cache_type != 2 && cache_type != 3) ||
            depth % (cache_type == 3 ? 16 : 8) || page_size < 1 || table_width < 0 || window < 0 || sinks < 0 ||
-           (long long)batch * heads_count > INT_MAX;
+           (long long)batch * heads_count > kMostHeads;
 }
 
 } // namespace attend

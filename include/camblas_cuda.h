@@ -513,11 +513,12 @@ int camblas_cuda_qk_norm_rope(camblas_cuda_context *context, int tokens, int hea
  * depth] BF16, output the same, contiguous. strides, in elements: {q batch, q
  * head, key page, key slot, key head, value page, value slot, value head, table
  * row}. depth a multiple of 8 up to 256 (of 16 for E4M3), heads a multiple of
- * kv_heads; q 8-byte aligned with strides multiples of 4, output 4-byte aligned,
- * caches 16-byte aligned with strides multiples of 16 bytes. workspace: device
- * memory of at least camblas_cuda_paged_attention_workspace bytes (0 for invalid
- * sizes), 16-byte aligned, used by this call only until it has run. No atomics:
- * the same call gives the same bits. Counter slot 6 counts it. */
+ * kv_heads, batch * heads at most 2^31 - 64; q 8-byte aligned with strides
+ * multiples of 4, output 4-byte aligned, caches 16-byte aligned with strides
+ * multiples of 16 bytes. workspace: device memory of at least
+ * camblas_cuda_paged_attention_workspace bytes (0 for invalid sizes), 16-byte
+ * aligned, used by this call only until it has run. No atomics: the same call
+ * gives the same bits. Counter slot 6 counts it. */
 size_t camblas_cuda_paged_attention_workspace(const camblas_cuda_context *context, int batch,
                                               int heads, int kv_heads, int depth, int cache_type,
                                               int page_size, int table_width, int window, int sinks);
