@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Scor
 #pragma unroll
     for (int i = 0; i < PerLane; ++i)
         group_of[i] = int((i * 32 + lane + 0.5f) * inverse);
-    for (int token = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; token < task.tokens; token += warps) {
+    /* 64 bits: the step behind the last token may leave 32 */
+    for (long long token = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; token < task.tokens; token += warps) {
         const T *row = static_cast<const T *>(task.logits) + token * task.ld_logits;
         float x[PerLane];
         float top = -INFINITY;
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Scor
                 total += shuffle_xor(total, offset);
         }
         if (chosen) {
-            const long long at = (long long)token * task.choices + lane;
+            const long long at = token * task.choices + lane;
             task.chosen[at] = mine;
             task.weights[at] = float((total != 0 ? score / total : 0.0) * double(task.scale));
         }

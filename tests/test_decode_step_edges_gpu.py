@@ -99,3 +99,18 @@ def test_attention_counts_its_sequences_in_32_bits(gen):
     assert status < 0 and "dimensions" in message
     status, message = attention_by_c(gen, batch=2 ** 29 - 16)  # a size that is taken, with too small a workspace
     assert status < 0 and "workspace" in message
+
+
+def test_router_at_the_largest_number_of_tokens():
+    """The step of the last warps passes 2^31."""
+    tokens = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 45 * 2 ** 30:
+        pytest.skip("needs 45 GB")
+    logits = torch.zeros(tokens, 1, dtype=BF16, device="cuda")
+    ids, weights = _kernels.route_experts(logits, 1, scoring="sigmoid", renormalise=False)
+    del logits
+    for start in range(0, tokens, 2 ** 28):
+        assert not ids[start:start + 2 ** 28].any()
+        assert (weights[start:start + 2 ** 28] == 0.5).all()
+    del ids, weights
+    torch.cuda.empty_cache()
