@@ -217,6 +217,11 @@ __device__ __forceinline__ bool surely_larger(float a, float b)
     return a - b > 0x1p-17f * (1.f + fabsf(a)); /* false for a NaN and for infinities */
 }
 
+/* How far the sum of a group's two largest ranks may be off, the larger of which has this magnitude: 2^-18
+ * for either score, 2^-24 of the magnitude for either sum with a bias and twice that for the sum of the
+ * two, which may be far smaller than they, and for taking the doubt from it: together below this. */
+__device__ __forceinline__ float group_doubt(float magnitude) { return 0x1p-17f + 0x1p-20f * magnitude; }
+
 template <int PerLane, typename T>
 __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ ScoreTask task)
 {
@@ -276,7 +281,8 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Scor
                 key[i] = e < task.experts ? key_of(score[i] + (task.bias ? task.bias[e] : 0.f)) : 0;
             }
             if (task.groups > 1) {
-                unsigned mine = 0; /* lane g: the rank of group g */
+                float mine = NAN; /* lane g: the rank of group g, and how far it may be off */
+                float doubt = 0.f;
 #pragma unroll 1
                 for (int group = 0; group < task.groups; ++group) {
                     unsigned first = 0, second = 0;
@@ -287,28 +293,31 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Scor
                         first = max(first, k);
                     }
                     const unsigned best = __reduce_max_sync(0xffffffffu, first);
-                    float rank = rank_of(best);
+                    float rank = rank_of(best), magnitude = fabsf(rank);
                     if (size > 1) {
                         /* the lane of the largest offers its next, the others their first */
                         const unsigned owners = __ballot_sync(0xffffffffu, first == best);
                         const unsigned offer = lane == __ffs(owners) - 1 ? second : first;
-                        rank += rank_of(__reduce_max_sync(0xffffffffu, offer));
+                        const float next = rank_of(__reduce_max_sync(0xffffffffu, offer));
+                        magnitude = fmaxf(magnitude, fabsf(next)), rank += next;
                     }
                     if (lane == group)
-                        mine = key_of(rank);
+                        mine = rank, doubt = group_doubt(magnitude);
                 }
                 unsigned keep = 0;
-                float last = 0.f;
-                unsigned one[1] = {mine};
+                unsigned one[1] = {lane < task.groups ? key_of(mine) : 0};
 #pragma unroll 1
                 for (int round = 0; round < task.kept; ++round) {
                     int at;
-                    last = rank_of(take_best(one, at));
+                    take_best(one, at);
                     keep |= 1u << (at & 31);
                 }
-                if (task.kept < task.groups) { /* twice the bound: a group's rank is a sum of two */
-                    const float next = rank_of(__reduce_max_sync(0xffffffffu, one[0]));
-                    certain = surely_larger(0.5f * last, 0.5f * next);
+                if (task.kept < task.groups) {
+                    const bool kept = (keep >> lane) & 1;
+                    const unsigned least = __reduce_min_sync(0xffffffffu, kept ? key_of(mine - doubt) : ~0u);
+                    const unsigned most =
+                        __reduce_max_sync(0xffffffffu, !kept && lane < task.groups ? key_of(mine + doubt) : 0);
+                    certain = rank_of(least) > rank_of(most); /* false for a NaN */
                 }
 #pragma unroll
                 for (int i = 0; i < PerLane; ++i)

@@ -114,3 +114,22 @@ def test_router_at_the_largest_number_of_tokens():
         assert (weights[start:start + 2 ** 28] == 0.5).all()
     del ids, weights
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_groups_whose_ranks_cancel(gen, scoring):
+    """Large biases of opposite sign in a group: the sum of its two ranks is small beside their rounding to FP32."""
+    logits = torch.tensor([[1.503, 0.286, 1.711, 0.170]], device="cuda")
+    bias = torch.tensor([1e4, -1e4, 1e4, -1e4], device="cuda")
+    options = dict(bias=bias, scoring=scoring, groups=2, kept_groups=1)
+    assert torch.equal(_kernels.route_experts(logits, 2, **options)[0].cpu(), exact.route(logits, 2, **options)[0])
+    for experts, groups, kept in ((64, 32, 5), (96, 8, 3), (512, 4, 1)):
+        logits = 1.5 * normal(gen, 60, experts)
+        for size in (1e2, 1e4, 3e6, 3e38):
+            bias = torch.where(torch.arange(experts, device="cuda") % 2 == 0, size, -size)
+            bias[experts // 2] = 0.25
+            options = dict(bias=bias, scoring=scoring, groups=groups, kept_groups=kept)
+            ids, weights = _kernels.route_experts(logits, 4, **options)
+            want_ids, want = exact.route(logits, 4, **options)
+            assert torch.equal(ids.cpu(), want_ids)
+            assert ((weights.cpu().double() - want).abs() <= (exact.U32 * 1.001 + 1e-12) * want.abs()).all()
