@@ -887,9 +887,9 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, epsilon, positions, table, 
     The caches are ``[pages, page size, kv_heads, depth]`` BF16 or FP8 E4M3 in any order of
     strides with unit stride along the depth. Token ``i`` is written to slot ``slots[i]`` (int64,
     ``page * page_size + place``); a slot outside the cache, or a position outside the table,
-    writes nothing; slots that are written must be distinct. An E4M3 cache receives
-    ``key / key_scale`` and ``value / value_scale``, rounded once from FP32, at most 448 in
-    magnitude. Returns the new queries.
+    writes nothing; slots that are written must be distinct. The caches receive
+    ``key / key_scale`` and ``value / value_scale``, rounded once from FP32, in E4M3 at most 448 in
+    magnitude; ``paged_attention`` takes the same scales. Returns the new queries.
     """
     return _rotate(q, k, v, q_weight, k_weight, epsilon, positions, table, interleaved, key_cache,
                    value_cache, slots, key_scale, value_scale)[0]
@@ -905,7 +905,8 @@ def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, windo
     ``table[b, t // page size]`` (int32); it is visible when ``t < lengths[b]`` (int32) and, with
     ``window > 0``, when it is one of the last ``window`` or of the first ``sinks`` tokens. A token
     whose page number is outside the cache is not visible, a sequence that sees nothing gives
-    zeros. The default scale is ``1 / sqrt(depth)``. The work is cut over the lengths found on the
+    zeros. Entries of the caches, of either type, stand for ``entry * key_scale`` and
+    ``entry * value_scale``. The default scale is ``1 / sqrt(depth)``. The work is cut over the lengths found on the
     device, so a captured call follows them; the same call gives the same bits.
     """
     _refuse_gradient(q, key_cache, value_cache)

@@ -8,8 +8,8 @@
  * with pair i = (i, i + rotary/2), or (2i, 2i+1) when interleaved, and cos/sin row
  * p of a table the caller computed (angles of far positions lose their
  * fraction in FP32, so they are not formed here). Everything between the load
- * and the store is FP32; the result is rounded once, to BF16 or, for an 8-bit
- * cache, from FP32 straight to E4M3.
+ * and the store is FP32; the result, divided by the scale of its cache, is rounded
+ * once, to BF16 or, for an 8-bit cache, from FP32 straight to E4M3.
  *
  * The reads and writes of the heads bound the kernel: seven operations per
  * element against four bytes, as long as issue keeps up: a head's eight elements
@@ -82,13 +82,11 @@ __device__ __forceinline__ void store_piece(__nv_bfloat16 *to, const Piece &p)
     *reinterpret_cast<uint2 *>(to) = raw;
 }
 
-/* value / scale, rounded to the nearest E4M3, at most 448 in magnitude */
-__device__ __forceinline__ void store_piece_e4m3(uint8_t *to, const Piece &p, float scale)
+/* rounded to the nearest E4M3, at most 448 in magnitude */
+__device__ __forceinline__ void store_piece_e4m3(uint8_t *to, const Piece &p)
 {
-    const uint32_t low = __nv_cvt_float2_to_fp8x2(make_float2(p.e[0] / scale, p.e[1] / scale),
-                                                  __NV_SATFINITE, __NV_E4M3);
-    const uint32_t high = __nv_cvt_float2_to_fp8x2(make_float2(p.e[2] / scale, p.e[3] / scale),
-                                                   __NV_SATFINITE, __NV_E4M3);
+    const uint32_t low = __nv_cvt_float2_to_fp8x2(make_float2(p.e[0], p.e[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t high = __nv_cvt_float2_to_fp8x2(make_float2(p.e[2], p.e[3]), __NV_SATFINITE, __NV_E4M3);
     *reinterpret_cast<uint32_t *>(to) = low | (high << 16);
 }
 
@@ -298,13 +296,17 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
         if (slot >= 0 && slot < task.slot_count)
             page = slot / task.page_size, place = slot - page * task.page_size;
     }
-    const auto cache = [&](const CacheLayout &to, int head, float scale, const Piece &a, const Piece &b) {
+    const auto cache = [&](const CacheLayout &to, int head, float scale, Piece a, Piece b) {
         if (page < 0)
             return;
+        if (scale != 1.f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                a.e[i] /= scale, b.e[i] /= scale;
         const long long at = page * to.page_stride + place * to.slot_stride + head * to.head_stride;
         if (task.eight_bit) {
             uint8_t *row = static_cast<uint8_t *>(to.base) + at;
-            store_piece_e4m3(row + first, a, scale), store_piece_e4m3(row + second, b, scale);
+            store_piece_e4m3(row + first, a), store_piece_e4m3(row + second, b);
         } else {
             __nv_bfloat16 *row = static_cast<__nv_bfloat16 *>(to.base) + at;
             store_piece(row + first, a), store_piece(row + second, b);

@@ -466,9 +466,9 @@ int camblas_cuda_reduce_groups(camblas_cuda_context *context, int tokens, int ch
  * is dense, single-head and cacheless (camblas_cuda.h:80-85) and whose expert
  * routing starts from ids (routing.cuh). A cache holds the keys (and another
  * the values) of all sequences in pages: [pages][page_size][kv_heads][depth],
- * any strides but unit stride along depth, cache_type 2 BF16 or 3 E4M3. An E4M3
- * entry stands for value = entry * scale, with one scale for the keys and one
- * for the values. */
+ * any strides but unit stride along depth, cache_type 2 BF16 or 3 E4M3. An entry
+ * of either type stands for value = entry * scale, with one scale for the keys and
+ * one for the values. */
 
 /* RMS norm of every query and key head with its weight, then the position
  * rotation, with one rounding:
@@ -484,9 +484,8 @@ int camblas_cuda_reduce_groups(camblas_cuda_context *context, int tokens, int ch
  * cache arguments are ignored. cache_type 2 or 3: keys and values go to slot
  * slots[token] (int64; page * page_size + place in the page) of the caches,
  * keys from the FP32 result divided by key_scale, values divided by
- * value_scale, saturating at 448 for E4M3 (with cache_type 2 both scales are
- * ignored); a slot outside [0, pages * page_size) is not written, slots that
- * are written must be distinct. k_out may then be NULL. strides, in elements:
+ * value_scale, saturating at 448 for E4M3; a slot outside [0, pages *
+ * page_size) is not written, slots that are written must be distinct. k_out may then be NULL. strides, in elements:
  * {q token, q head, k token, k head, v token, v head, key page, key slot, key
  * head, value page, value slot, value head}, the last eight only with a cache.
  * depth a multiple of 8 up to 256, rotary a multiple of 8 up to depth; q, k, v,

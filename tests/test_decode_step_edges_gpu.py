@@ -133,3 +133,39 @@ def test_groups_whose_ranks_cancel(gen, scoring):
             want_ids, want = exact.route(logits, 4, **options)
             assert torch.equal(ids.cpu(), want_ids)
             assert ((weights.cpu().double() - want).abs() <= (exact.U32 * 1.001 + 1e-12) * want.abs()).all()
+
+
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+def test_cache_scales_mean_the_same_to_the_writer_and_the_reader(gen, kind):
+    """value = entry * scale for either type of cache: what was appended under scales is attended over under them."""
+    tokens, page, kv_heads, depth = 9, 4, 2, 64
+    q, k, v = (normal(gen, tokens, n, depth).to(BF16) for n in (4, kv_heads, kv_heads))
+    w = (1 + 0.3 * normal(gen, depth)).to(BF16)
+    positions, slots = torch.arange(tokens, device="cuda"), torch.randperm(12, generator=gen, device="cuda")[:tokens]
+    table = _kernels.rotary_table(16, depth)
+    keys, values = (torch.zeros(3, page, kv_heads, depth, device="cuda").to(kind) for _ in range(2))
+    scales = dict(key_scale=0.037, value_scale=0.0625 / 3)
+    _kernels.qk_norm_rope_append(q, k, v, w, w, 1e-5, positions, table, keys, values, slots, **scales)
+    new, bound = exact.norm_rope(k, w, 1e-5, positions, table, False)
+    for cache, want, room, scale in ((keys, new, bound, scales["key_scale"]),
+                                     (values, v.double(), torch.zeros_like(bound), scales["value_scale"])):
+        entry = want / scale
+        # the quotient adds a unit of FP32 and the scale's own rounding one; E4M3 has a fixed step below 2^-6
+        room = room / scale + 3 * exact.U32 * entry.abs() + (2.0 ** -10 if kind == E4M3 else 0.0)
+        got = cache.view(torch.uint8).flatten(0, 1)[slots].view(kind) if kind == E4M3 else cache.flatten(0, 1)[slots]
+        assert exact.within(got, entry.clamp(-448, 448) if kind == E4M3 else entry, room)
+    pages = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    counts = torch.tensor([12], dtype=torch.int32, device="cuda")
+    out = _kernels.paged_attention(q[:1], keys, values, pages, counts, **scales)
+    want, bound = exact.attention(q[:1], keys, values, pages, counts, depth ** -0.5, 0, 0, **scales)
+    assert exact.within(out, want, bound + 4 * exact.U32 * want.abs())
+
+
+def test_scales_of_one_change_no_bit_of_a_cache(gen):
+    q, k, v = (normal(gen, 5, n, 80).to(BF16) for n in (2, 1, 1))
+    positions = torch.arange(5, device="cuda")
+    table = _kernels.rotary_table(8, 80)
+    keys, values = (torch.zeros(2, 4, 1, 80, device="cuda", dtype=BF16) for _ in range(2))
+    _kernels.qk_norm_rope_append(q, k, v, None, None, 0.0, positions, table, keys, values, positions)
+    assert torch.equal(values.flatten(0, 1)[:5], v)
+    assert torch.equal(keys.flatten(0, 1)[:5], _kernels.qk_norm_rope(q, k, None, None, 0.0, positions, table)[1])
