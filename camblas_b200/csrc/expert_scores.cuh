@@ -11,12 +11,13 @@
  * Equal ranks go to the lower index, and a NaN ranks behind every number.
  *
  * Which expert is chosen is a whole number that no tolerance covers, and ranks
- * may lie closer than FP32 can tell. Without bias and groups the logits
- * themselves are compared: both scores grow with them. Otherwise the choice is
- * made on FP32 ranks, whose error is bounded, and made again on FP64 ranks for a
+ * may lie closer than FP32 can tell: they are compared in FP64. Without bias and
+ * groups the choice is made on the logits themselves, with which both scores grow;
+ * otherwise on FP32 ranks, whose error is bounded. It is made again on FP64 ranks for a
  * token where two ranks that decide anything lie within that bound (a few
  * tokens in a thousand; every FP64 exponential costs some forty instructions of a
- * rate of one in two). The weights are FP64 throughout, which is cheap for the
+ * rate of one in two), or where distinct logits that decide anything may have one
+ * FP64 score (saturated sigmoids, exponentials that underflow). The weights are FP64 throughout, which is cheap for the
  * chosen few: renormalised softmax weights do not need the sum over all.
  *
  * One warp per token, expert e on lane e % 32; a round of the choice is a local
@@ -80,6 +81,13 @@ __device__ __forceinline__ void warp_best(long long &key, int &index)
     }
 }
 
+/* exp(x) for x <= 0, rounded to nearest among FP64's subnormal numbers too, where exp may be off by a unit,
+ * which there can be all of it: 2^64 times as large first. */
+__device__ __forceinline__ double falling_exponential(double x)
+{
+    return x < -700.0 ? exp(x + 44.361419555836498) * 0x1p-64 : exp(x);
+}
+
 /* Lane j < choices: the j-th expert by FP64 ranks. */
 template <int PerLane>
 __device__ __noinline__ int choose_exactly(const ScoreTask &task, const float (&x)[PerLane], float top)
@@ -89,7 +97,7 @@ __device__ __noinline__ int choose_exactly(const ScoreTask &task, const float (&
     long long key[PerLane];
 #pragma unroll
     for (int i = 0; i < PerLane; ++i) {
-        score[i] = task.sigmoid ? 1.0 / (1.0 + exp(-double(x[i]))) : exp(double(x[i]) - top);
+        score[i] = task.sigmoid ? 1.0 / (1.0 + exp(-double(x[i]))) : falling_exponential(double(x[i]) - top);
         sum += score[i];
     }
     if (!task.sigmoid) {
@@ -222,6 +230,15 @@ __device__ __forceinline__ bool surely_larger(float a, float b)
  * two, which may be far smaller than they, and for taking the doubt from it: together below this. */
 __device__ __forceinline__ float group_doubt(float magnitude) { return 0x1p-17f + 0x1p-20f * magnitude; }
 
+/* Whether the scores of two logits, the larger first, are in the same order in FP64, and equal only where
+ * the logits are. From 2^-25 apart the exponentials differ by that relative to them, and by far more than
+ * FP64 rounds off, as long as the larger score is a normal number (`base` is the
+ * largest logit, for a sigmoid 0) and the 1 that a sigmoid adds to its exponential does not cover it. */
+__device__ __forceinline__ bool scores_ordered(float larger, float smaller, float base, bool sigmoid)
+{
+    return larger == smaller || (larger - smaller > 0x1p-25f && larger - base > -700.f && !(sigmoid && larger > 16.f));
+}
+
 template <int PerLane, typename T>
 __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ ScoreTask task)
 {
@@ -328,23 +345,33 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Scor
         int mine = 0;
         if (certain) {
             float before = INFINITY;
+            unsigned taken = 0; /* lane j: the key of its choice */
 #pragma unroll 1
             for (int round = 0; round < task.choices; ++round) {
                 int index;
-                const float rank = rank_of(take_best(key, index));
-                if (!by_logits)
+                const unsigned best = take_best(key, index);
+                if (!by_logits) {
+                    const float rank = rank_of(best);
                     certain = certain && (round == 0 ? rank == rank : surely_larger(before, rank));
-                before = rank;
+                    before = rank;
+                }
                 if (lane == round)
-                    mine = index;
+                    mine = index, taken = best;
             }
-            if (!by_logits) { /* the first that was not chosen */
-                unsigned next = 0;
+            /* the first that was not chosen */
+            unsigned next = 0;
 #pragma unroll
-                for (int i = 0; i < PerLane; ++i)
-                    next = max(next, key[i]);
-                next = __reduce_max_sync(0xffffffffu, next);
+            for (int i = 0; i < PerLane; ++i)
+                next = max(next, key[i]);
+            next = __reduce_max_sync(0xffffffffu, next);
+            if (!by_logits) {
                 certain = certain && (next == 0 || surely_larger(before, rank_of(next)));
+            } else { /* lane j: its choice after the one before it; lane 0: the first not chosen after the last */
+                const unsigned larger = __shfl_sync(0xffffffffu, taken, lane == 0 ? task.choices - 1 : lane - 1);
+                const unsigned smaller = lane == 0 ? next : taken;
+                certain = __all_sync(0xffffffffu, lane >= task.choices || smaller == 0 ||
+                                                      scores_ordered(rank_of(larger), rank_of(smaller),
+                                                                     task.sigmoid ? 0.f : top, task.sigmoid));
             }
         }
         if (!certain)

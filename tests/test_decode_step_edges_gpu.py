@@ -169,3 +169,36 @@ def test_scales_of_one_change_no_bit_of_a_cache(gen):
     _kernels.qk_norm_rope_append(q, k, v, None, None, 0.0, positions, table, keys, values, positions)
     assert torch.equal(values.flatten(0, 1)[:5], v)
     assert torch.equal(keys.flatten(0, 1)[:5], _kernels.qk_norm_rope(q, k, None, None, 0.0, positions, table)[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_distinct_logits_of_equal_scores(gen, dtype):
+    """Ranks are compared in FP64, where distinct logits can have one score: the lower index comes first, with a
+    bias of zeros as without one."""
+    inf = float("inf")
+    sigmoid = [[40.0, 45.0, 1.0, 60.0], [1e-20, 2e-20, 0.0, -1.0], [-800.0, -750.0, -900.0, -710.0],
+               [-inf, -800.0, -inf, 2.0], [15.0, 15.5, 16.0, 16.5], [39.0, 38.5, 38.0, 37.0]]
+    softmax = [[0.0, -900.0, -800.0, -1.0], [0.0, 1e-20, -1e-20, 3e-20], [100.0, -640.0, -647.0, -800.0],
+               [-inf, -800.0, 0.0, -750.0], [1000.0, 1.0, 2.0, 3.0], [5.0, 5.5, 6.0, 6.5]]
+    for scoring, rows in (("sigmoid", sigmoid), ("softmax", softmax)):
+        logits = torch.tensor(rows, device="cuda").to(dtype)
+        for experts in (4, 40, 300):
+            wide = torch.full((len(rows), experts), -inf, device="cuda", dtype=dtype)
+            wide[:, torch.arange(4) * (experts // 4)] = logits
+            for choices in (1, 2, 3, 4):
+                ids, weights = _kernels.route_experts(wide, choices, scoring=scoring)
+                want_ids, want = exact.route(wide, choices, scoring=scoring)
+                assert torch.equal(ids.cpu(), want_ids)
+                # below FP32's normal numbers the step is 2^-149, and a rounding off by up to half of it
+                room = (exact.U32 * 1.001 + 1e-12) * want.abs() + 2.0 ** -150
+                assert ((weights.cpu().double() - want).abs() <= room).all()
+                zero = _kernels.route_experts(wide, choices, bias=torch.zeros(experts, device="cuda"), scoring=scoring)
+                assert torch.equal(zero[0], ids) and torch.equal(zero[1], weights)
+
+
+@pytest.mark.parametrize("scoring,spread", [("softmax", 400.0), ("sigmoid", 15.0), ("softmax", 1e-12)])
+def test_saturated_scores_of_many_experts(gen, scoring, spread):
+    logits = spread * normal(gen, 40, 128)
+    for choices in (1, 8, 32):
+        ids, _ = _kernels.route_experts(logits, choices, scoring=scoring)
+        assert torch.equal(ids.cpu(), exact.route(logits, choices, scoring=scoring)[0])
