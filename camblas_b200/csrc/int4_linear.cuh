@@ -4,8 +4,8 @@
  *   out[r,o] = sum over groups G of s[o,G] * sum_{k in G} (c[o,k] - z[o,G]) x[r,k]
  *              (+ bias[o]) (+ residual[r,o]),
  * codes c and zero points z in 0..15 (z = 8 without zero points), groups of 32,
- * 64 or 128 input features. c - z is a whole number of at most 15 and exact in
- * BF16, so the products run on the tensor cores over exact operands; the FP32
+ * 64 or 128 input features. c - z is a whole number of at most 15, exact in 16
+ * bits, so the products run on the tensor cores over exact operands; the FP32
  * sums of a group are scaled in FP32, and the result is rounded once. Scaling
  * the weights themselves to BF16 before the product would round each of them.
  *
@@ -19,21 +19,20 @@
  *
  * Unpacking. A nibble n, alone in the low bits of an FP16, is the subnormal
  * n * 2^-24, exact, and in the next four bits 16 n * 2^-24; so a pair of codes is
- * one AND of the word, or of the word shifted by 8, and five instructions unpack
- * a product's operand. (128 + n in BF16, less 128 + z, takes eleven, and then
- * issue and not HBM is the bound: 70 us for one token, 28672 -> 8192, where this
- * takes 30.) The factors 2^24 and 1/16 go to the scales,
- * and the zero point is taken out of the group's sum in FP32:
- *   sum (c - z) x = sum c x - z sum x.
+ * one AND of the word, or of the word shifted by 8, and the zero point, in the same
+ * form, is subtracted from both at once, which is exact: nine instructions for a
+ * product's operand. The factors 2^24 and 1/16 go to the scales. (128 + n in BF16,
+ * less 128 + z, takes eleven: 70 us for one token, 28672 -> 8192, where this takes
+ * 30. Taking z sum x from a group's sum of c x afterwards takes five, but what is
+ * left where c is near z is the rounding of sums that are far larger.)
  *
  * The tokens are brought to FP16 first, in a small kernel of their own:
  * spread_tokens multiplies each 128 inputs of a token by a power of two that
  * brings the largest to [2^14, 2^15), where an FP16 holds a BF16 exactly down to
  * 2^-31 of the largest (its least step is 2^-24, a BF16's 2^-7 of its own power of
- * two) and below that to within 2^-39 of it, and leaves the power and the sum
- * of every group. The product is its programmatic dependent and has its first
+ * two) and below that to within 2^-39 of it, and leaves the power. The product is its programmatic dependent and has its first
  * weights in flight before it waits for the tokens. A token element that
- * is infinite or NaN makes the token's outputs NaN.
+ * is infinite or NaN makes the power, and so the token's outputs, NaN.
  *
  * Layout: [block of 64 outputs][unit of 128 inputs][4 tiles of 16 outputs], a
  * tile of a unit being 1024 bytes of codes, then its scales, then its zero points
@@ -69,25 +68,24 @@ struct LinearTask {
     long long ldr;
     __nv_bfloat16 *out;
     long long ldo;
-    /* Workspace. Tokens are taken in passes of `pass_rows`; for every unit a pass has the factors
-     * of its tokens (their powers, then for each group the sums times 2^-24, pass_rows of each)
-     * and then its tokens in FP16, 256 bytes each. Odd tokens have the 64-byte halves of each 128
+    /* Workspace. Tokens are taken in passes of `pass_rows`; for every unit a pass has the powers
+     * of its tokens, pass_rows of them, and then its tokens in FP16, 256 bytes each. Odd tokens have the 64-byte halves of each 128
      * bytes swapped, so that the operand reads of two tokens meet different banks. */
     int pass_rows;
     uint8_t *tokens;
     unsigned *status;
 };
 
-/* Bytes of a tile of a unit, and of a unit's factors. */
+/* Bytes of a tile of a unit, and of a unit's powers. */
 template <int Group, typename Scale, bool Zeros> __host__ __device__ constexpr int tile_bytes()
 {
     return 16 * kUnit / 2 + kUnit / Group * 16 * (int(sizeof(Scale)) + (Zeros ? 1 : 0));
 }
 
-__host__ __device__ constexpr int factor_bytes(int group, int rows) { return (1 + kUnit / group) * rows * 4; }
+__host__ __device__ constexpr int power_bytes(int rows) { return rows * 4; }
 
 /* One warp per unit of a token: 16 lanes with eight inputs each, two units per warp. */
-template <int Group> __global__ void __launch_bounds__(256) spread_tokens(const __grid_constant__ LinearTask task)
+__global__ void __launch_bounds__(256) spread_tokens(const __grid_constant__ LinearTask task)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x % 32, piece = lane % 16;
@@ -101,12 +99,16 @@ template <int Group> __global__ void __launch_bounds__(256) spread_tokens(const 
     const heads::Piece low = heads::unpack_piece(make_uint2(raw.x, raw.y));
     const heads::Piece high = heads::unpack_piece(make_uint2(raw.z, raw.w));
     float largest = 0.f;
+    bool broken = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
         largest = fmaxf(largest, fmaxf(fabsf(low.e[i]), fabsf(high.e[i])));
+        broken = broken || !(fabsf(low.e[i]) < INFINITY) || !(fabsf(high.e[i]) < INFINITY);
+    }
 #pragma unroll
     for (int offset = 1; offset < 16; offset *= 2)
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
+    const unsigned broken_lanes = __ballot_sync(0xffffffffu, broken) >> (lane & 16) & 0xffff; /* of this unit */
     const int exponent = attend::half_exponent(largest);
     const float down = __int_as_float((127 - exponent) << 23), up = __int_as_float((127 + exponent) << 23);
     uint4 halves;
@@ -114,37 +116,43 @@ template <int Group> __global__ void __launch_bounds__(256) spread_tokens(const 
     halves.y = attend::pack<true>(low.e[2] * down, low.e[3] * down);
     halves.z = attend::pack<true>(high.e[0] * down, high.e[1] * down);
     halves.w = attend::pack<true>(high.e[2] * down, high.e[3] * down);
-    float sum = 0.f;
-    const uint32_t words[4] = {halves.x, halves.y, halves.z, halves.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 pair = __half22float2(*reinterpret_cast<const __half2 *>(&words[i]));
-        sum += pair.x + pair.y;
-    }
-#pragma unroll
-    for (int offset = 1; offset < Group / 8; offset *= 2)
-        sum += __shfl_xor_sync(0xffffffffu, sum, offset);
     if (!live)
         return;
     const int pass = row / task.pass_rows, column = row - pass * task.pass_rows;
     const int pass_live = min(task.pass_rows, task.rows - pass * task.pass_rows);
-    const int ahead = factor_bytes(Group, task.pass_rows);
+    const int ahead = power_bytes(task.pass_rows);
     uint8_t *base = task.tokens + (long long)pass * task.units * (ahead + task.pass_rows * kTokenBytes) +
                     (long long)unit * (ahead + pass_live * kTokenBytes);
     *reinterpret_cast<uint4 *>(base + ahead + column * kTokenBytes + (piece ^ (column & 1) * 4) * 16) = halves;
-    float *factors = reinterpret_cast<float *>(base) + column;
     if (piece == 0)
-        *factors = up;
-    if (piece % (Group / 8) == 0)
-        factors[(1 + piece / (Group / 8)) * task.pass_rows] = sum * 0x1p-24f;
+        reinterpret_cast<float *>(base)[column] = broken_lanes ? NAN : up;
 }
 
-/* Row operand of one product: registers 0 and 2 are 2^-24 times the codes of
- * output g, 1 and 3 are 2^-20 times those of output g + 8. */
-__device__ __forceinline__ void unpack(uint32_t (&a)[4], uint32_t word)
+/* A zero point of output g and of g + 8 as an operand's codes have theirs, twice. */
+struct ZeroPair {
+    uint32_t low, high;
+};
+
+__device__ __forceinline__ ZeroPair zero_pair(uint32_t two_bytes)
 {
-    a[0] = word & 0x000f000fu, a[1] = word & 0x00f000f0u;
-    a[2] = (word >> 8) & 0x000f000fu, a[3] = (word >> 8) & 0x00f000f0u;
+    return {(two_bytes & 0xff) * 0x00010001u, (two_bytes >> 8) * 0x00100010u};
+}
+
+constexpr uint32_t kNoZeros = 0x0808; /* the zero points without any */
+
+__device__ __forceinline__ uint32_t subtract(uint32_t codes, uint32_t zeros)
+{
+    uint32_t r; /* exact: subnormal numbers, which this form does not flush */
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(codes), "r"(zeros));
+    return r;
+}
+
+/* Row operand of one product: registers 0 and 2 are 2^-24 times the codes less the
+ * zero point of output g, 1 and 3 are 2^-20 times those of output g + 8. */
+__device__ __forceinline__ void unpack(uint32_t (&a)[4], uint32_t word, const ZeroPair &zero)
+{
+    a[0] = subtract(word & 0x000f000fu, zero.low), a[1] = subtract(word & 0x00f000f0u, zero.high);
+    a[2] = subtract((word >> 8) & 0x000f000fu, zero.low), a[3] = subtract((word >> 8) & 0x00f000f0u, zero.high);
 }
 
 __device__ __forceinline__ float2 scale_pair(const float *from) { return *reinterpret_cast<const float2 *>(from); }
@@ -156,14 +164,6 @@ __device__ __forceinline__ float2 scale_pair(const __nv_bfloat16 *from)
 /* The scales of outputs g and g + 8 with the factors of their codes taken back, before a token's power
  * comes in: a small power times 2^-24 would leave FP32's normal numbers. */
 __device__ __forceinline__ float2 raised(float2 scales) { return make_float2(scales.x * 0x1p24f, scales.y * 0x1p20f); }
-
-/* Zero points of outputs g and g + 8, the second times 16 like its codes; a byte in the low bits of
- * 2^23 is that number. */
-__device__ __forceinline__ float2 zero_pair(uint32_t two_bytes)
-{
-    return make_float2(__uint_as_float(0x4b000000u | (two_bytes & 0xff)) - 0x1p23f,
-                       __uint_as_float(0x4b000000u | (two_bytes >> 4 & 0xff0)) - 0x1p23f);
-}
 
 /* C = 0 form of the product, for the first of a group. */
 __device__ __forceinline__ void multiply_fresh(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -196,7 +196,7 @@ __device__ __forceinline__ void bulk_load(uint32_t to, const void *from, uint32_
 }
 
 /* What a stage of the ring holds: kUnits units of 64 outputs' weights, then of the
- * factors and tokens of the pass, `live` tokens each. */
+ * powers and tokens of the pass, `live` tokens each. */
 template <int Columns, int Group, typename Scale, bool Zeros> struct Stage {
     static constexpr int kGroups = kUnit / Group;
     static constexpr int kTokens = 8 * Columns;
@@ -204,7 +204,7 @@ template <int Columns, int Group, typename Scale, bool Zeros> struct Stage {
     static constexpr int kStages = Columns > 2 ? 3 : 4;
     static constexpr int kTileBytes = tile_bytes<Group, Scale, Zeros>();
     static constexpr int kScalesAt = 16 * kUnit / 2, kZerosAt = kScalesAt + kGroups * 16 * int(sizeof(Scale));
-    static constexpr int kFactorBytes = factor_bytes(Group, kTokens);
+    static constexpr int kPowerBytes = power_bytes(kTokens);
     static constexpr int kTokensAt = kUnits * kWarps * kTileBytes;
     /* The sums that the cluster exchanges, [token][output]: a warp reads 128 contiguous bytes of
      * another CTA (lane by lane from rows of their own took 12 us of 39 at 37 tokens, 42 of 66 at
@@ -213,7 +213,7 @@ template <int Columns, int Group, typename Scale, bool Zeros> struct Stage {
     static constexpr int kExchange = kTokens * kPitch * 4;
     static constexpr int kFitRegisters = Columns > 2 ? 3 : (Columns > 1 ? 5 : 7); /* CTAs on an SM */
 
-    static __host__ __device__ constexpr int pass_bytes(int live) { return kFactorBytes + live * kTokenBytes; }
+    static __host__ __device__ constexpr int pass_bytes(int live) { return kPowerBytes + live * kTokenBytes; }
     static __host__ __device__ constexpr int bytes(int live) { return kTokensAt + kUnits * pass_bytes(live); }
     /* The ring; then room for the tokens that the last stage's columns without a token read (what
      * they give goes nowhere), so that every read stays in the allocation; then the barriers. */
@@ -327,8 +327,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
                     break;
                 const uint8_t *own = held + (u * kWarps + warp) * S::kTileBytes;
                 const uint8_t *pass_unit = held + S::kTokensAt + u * S::pass_bytes(live);
-                const uint8_t *token = pass_unit + S::kFactorBytes + g * kTokenBytes + 16 * t;
-                const float *factor = reinterpret_cast<const float *>(pass_unit) + 2 * t;
+                const uint8_t *token = pass_unit + S::kPowerBytes + g * kTokenBytes + 16 * t;
+                const float *powers = reinterpret_cast<const float *>(pass_unit) + 2 * t;
                 float part_sum[Columns][4]; /* of outputs g (0, 1) and g + 8, before the token's power */
 #pragma unroll
                 for (int n = 0; n < Columns; ++n)
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
                 for (int i = 0; i < kGroups; ++i) {
                     const float2 s =
                         raised(scale_pair(reinterpret_cast<const Scale *>(own + S::kScalesAt) + 16 * i + 2 * g));
-                    float2 z = make_float2(8.f, 128.f);
+                    ZeroPair z = zero_pair(kNoZeros);
                     if constexpr (Zeros)
                         z = zero_pair(*reinterpret_cast<const uint16_t *>(own + S::kZerosAt + 16 * i + 2 * g));
                     float part[Columns][4];
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
                         if (piece % 2 == 0)
                             words = *reinterpret_cast<const uint4 *>(own + 512 * (piece / 2) + 16 * lane);
                         uint32_t a[2][4];
-                        unpack(a[0], piece % 2 ? words.z : words.x), unpack(a[1], piece % 2 ? words.w : words.y);
+                        unpack(a[0], piece % 2 ? words.z : words.x, z), unpack(a[1], piece % 2 ? words.w : words.y, z);
 #pragma unroll
                         for (int n = 0; n < Columns; ++n) {
                             const uint4 in = *reinterpret_cast<const uint4 *>(
@@ -362,16 +362,15 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Stage<Columns, Group, Scale,
                     }
 #pragma unroll
                     for (int n = 0; n < Columns; ++n) {
-                        const float2 taken = *reinterpret_cast<const float2 *>(factor + (1 + i) * S::kTokens + 8 * n);
-                        part_sum[n][0] = fmaf(s.x, fmaf(-z.x, taken.x, part[n][0]), part_sum[n][0]);
-                        part_sum[n][1] = fmaf(s.x, fmaf(-z.x, taken.y, part[n][1]), part_sum[n][1]);
-                        part_sum[n][2] = fmaf(s.y, fmaf(-z.y, taken.x, part[n][2]), part_sum[n][2]);
-                        part_sum[n][3] = fmaf(s.y, fmaf(-z.y, taken.y, part[n][3]), part_sum[n][3]);
+                        part_sum[n][0] = fmaf(s.x, part[n][0], part_sum[n][0]);
+                        part_sum[n][1] = fmaf(s.x, part[n][1], part_sum[n][1]);
+                        part_sum[n][2] = fmaf(s.y, part[n][2], part_sum[n][2]);
+                        part_sum[n][3] = fmaf(s.y, part[n][3], part_sum[n][3]);
                     }
                 }
 #pragma unroll
                 for (int n = 0; n < Columns; ++n) {
-                    const float2 power = *reinterpret_cast<const float2 *>(factor + 8 * n);
+                    const float2 power = *reinterpret_cast<const float2 *>(powers + 8 * n);
                     sum[n][0] = fmaf(power.x, part_sum[n][0], sum[n][0]), sum[n][1] = fmaf(power.y, part_sum[n][1], sum[n][1]);
                     sum[n][2] = fmaf(power.x, part_sum[n][2], sum[n][2]), sum[n][3] = fmaf(power.y, part_sum[n][3], sum[n][3]);
                 }
@@ -484,9 +483,9 @@ __global__ void __launch_bounds__(kWarps * 32, 7) few_kernel(const __grid_consta
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const int row = min(g, task.rows - 1); /* columns behind the last token repeat it */
-    const int pitch = factor_bytes(Group, 8) + task.rows * kTokenBytes;
+    const int pitch = power_bytes(8) + task.rows * kTokenBytes;
     const uint8_t *unit_tokens = task.tokens + (long long)begin * pitch;
-    const int token_at = factor_bytes(Group, 8) + row * kTokenBytes + 16 * t, swap = row & 1;
+    const int token_at = power_bytes(8) + row * kTokenBytes + 16 * t, swap = row & 1;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     for (int base = begin; base < end; base += kAhead) {
 #pragma unroll
@@ -497,12 +496,13 @@ __global__ void __launch_bounds__(kWarps * 32, 7) few_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 in[i] = *reinterpret_cast<const uint4 *>(unit_tokens + token_at + 64 * (i ^ swap));
-            const float *factor = reinterpret_cast<const float *>(unit_tokens) + 2 * t;
-            const float2 power = *reinterpret_cast<const float2 *>(factor);
+            const float2 power = *reinterpret_cast<const float2 *>(unit_tokens + 8 * t);
             float2 low = make_float2(0.f, 0.f), high = make_float2(0.f, 0.f); /* outputs g and g + 8 */
 #pragma unroll
             for (int i = 0; i < kGroups; ++i) {
-                const float2 taken = *reinterpret_cast<const float2 *>(factor + (1 + i) * 8);
+                ZeroPair z = zero_pair(kNoZeros);
+                if constexpr (Zeros)
+                    z = zero_pair(held[d].zeros[i]);
                 float part_sum[kPerGroup > 2 ? 2 : 1][4];
 #pragma unroll
                 for (int j = 0; j < kPerGroup; ++j) {
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32, 7) few_kernel(const __grid_consta
                     const uint32_t word = product % 4 == 0 ? w.x : (product % 4 == 1 ? w.y : (product % 4 == 2 ? w.z : w.w));
                     const uint32_t b0 = product % 2 ? v.z : v.x, b1 = product % 2 ? v.w : v.y;
                     uint32_t a[4];
-                    unpack(a, word);
+                    unpack(a, word, z);
                     if (j == chain)
                         multiply_fresh(part_sum[chain], a, b0, b1);
                     else
@@ -522,14 +522,9 @@ __global__ void __launch_bounds__(kWarps * 32, 7) few_kernel(const __grid_consta
                     for (int e = 0; e < 4; ++e)
                         part_sum[0][e] += part_sum[1][e];
                 }
-                float2 z = make_float2(8.f, 128.f);
-                if constexpr (Zeros)
-                    z = zero_pair(held[d].zeros[i]);
                 const float2 s = raised(make_float2(float(held[d].scales[i].low), float(held[d].scales[i].high)));
-                low.x = fmaf(s.x, fmaf(-z.x, taken.x, part_sum[0][0]), low.x);
-                low.y = fmaf(s.x, fmaf(-z.x, taken.y, part_sum[0][1]), low.y);
-                high.x = fmaf(s.y, fmaf(-z.y, taken.x, part_sum[0][2]), high.x);
-                high.y = fmaf(s.y, fmaf(-z.y, taken.y, part_sum[0][3]), high.y);
+                low.x = fmaf(s.x, part_sum[0][0], low.x), low.y = fmaf(s.x, part_sum[0][1], low.y);
+                high.x = fmaf(s.y, part_sum[0][2], high.x), high.y = fmaf(s.y, part_sum[0][3], high.y);
             }
             fetch(held[d], base + d + kAhead);
             sum[0] = fmaf(power.x, low.x, sum[0]), sum[1] = fmaf(power.y, low.y, sum[1]);
@@ -713,7 +708,7 @@ cudaError_t launch_rows(camblas_cuda_context *context, const LinearTask &task, b
 template <int Group> int run(camblas_cuda_context *context, const LinearTask &task, int scale_type, bool zeros)
 {
     const dim3 grid((task.units + 15) / 16, task.rows);
-    spread_tokens<Group><<<grid, 256, 0, context->stream>>>(task);
+    spread_tokens<<<grid, 256, 0, context->stream>>>(task);
     int status = host::launched(context, "4-bit linear tokens");
     if (status != 0)
         return status;
@@ -737,11 +732,11 @@ inline int rows_of_pass(int rows)
     return rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 48 ? 48 : 64)));
 }
 
-inline size_t workspace_bytes(int rows, int inner, int group)
+inline size_t workspace_bytes(int rows, int inner)
 {
     const size_t units = (inner + kUnit - 1) / kUnit, pass_rows = rows_of_pass(rows);
     const size_t passes = (rows + pass_rows - 1) / pass_rows;
-    return units * (passes * factor_bytes(group, int(pass_rows)) + size_t(rows) * kTokenBytes);
+    return units * (passes * power_bytes(int(pass_rows)) + size_t(rows) * kTokenBytes);
 }
 
 } // namespace nibble
@@ -751,7 +746,7 @@ extern "C" size_t camblas_cuda_int4_linear_workspace(const camblas_cuda_context 
 {
     if (!context || rows == 0 || nibble::sizes_bad(rows, inner, group))
         return 0;
-    return nibble::workspace_bytes(rows, inner, group);
+    return nibble::workspace_bytes(rows, inner);
 }
 
 extern "C" int camblas_cuda_int4_linear(camblas_cuda_context *context, int rows, int inner, int outputs,
@@ -771,7 +766,7 @@ extern "C" int camblas_cuda_int4_linear(camblas_cuda_context *context, int rows,
             heads::misaligned(weights, 16) || heads::misaligned(bias, 2) || heads::misaligned(residual, 2) ||
             heads::misaligned(out, 2) || out == x || out == weights || (bias && out == bias))
             return host::fail(context, "invalid 4-bit linear operands", 1);
-        if (!workspace || workspace_bytes < nibble::workspace_bytes(rows, inner, group) ||
+        if (!workspace || workspace_bytes < nibble::workspace_bytes(rows, inner) ||
             heads::misaligned(workspace, 16) || workspace == out)
             return host::fail(context, "4-bit linear workspace too small", 1);
         nibble::LinearTask task{};

@@ -202,3 +202,25 @@ def test_saturated_scores_of_many_experts(gen, scoring, spread):
     for choices in (1, 8, 32):
         ids, _ = _kernels.route_experts(logits, choices, scoring=scoring)
         assert torch.equal(ids.cpu(), exact.route(logits, choices, scoring=scoring)[0])
+
+
+@pytest.mark.parametrize("rows", [1, 8, 13, 40, 64, 70])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, True), (128, True), (128, False)])
+def test_int4_codes_at_and_near_the_zero_point(gen, rows, group, zeros):
+    """What the zero point takes away leaves no noise: rows of codes equal to it give zeros, rows within one of it
+    keep the accuracy of their small weights, and a large input on a weight of zero leaves the others alone."""
+    outputs, inner = 150, 512
+    _, scale, zero = int4_case(gen, outputs, inner, group, True)
+    if not zeros:
+        zero = torch.full_like(zero, 8)
+    whole = zero.int().repeat_interleave(group, 1)
+    whole[50:100] = (whole[50:100] + integers(gen, -1, 2, 50, inner)).clamp(0, 15)
+    whole[100:] = integers(gen, 0, 16, 50, inner).int()
+    whole[100:, 77] = zero[100:, 77 // group].int()
+    codes = (whole[:, ::2] + 16 * whole[:, 1::2]).to(torch.uint8)
+    weight = _kernels.Int4Weight(codes, scale, zero if zeros else None)
+    x = normal(gen, rows, inner).to(BF16)
+    x[:, 77] = 2.0 ** 14
+    out = _kernels.int4_linear(x, weight)
+    assert not out[:, :50].any()
+    assert exact.within(out, *exact.int4(x, codes, scale, zero))
