@@ -224,6 +224,20 @@ template <int Columns, int Group, typename Scale, bool Zeros> struct Stage {
                    : (kExchange + 15) / 16 * 16;
     }
     static __host__ __device__ constexpr int shared(int live) { return ring(live) + 16 * kStages + 16; }
+    /* Whether every read of the products from the last stage, for columns without a token too, lies in
+     * the ring, and a launch asks for no more than allow_shared_kernel does. A later pass of fewer tokens
+     * reads less far in the ring of a full one. */
+    static constexpr bool reads_inside()
+    {
+        for (int live = 1; live <= kTokens; ++live) {
+            const int last_unit = (kStages - 1) * bytes(live) + kTokensAt + (kUnits - 1) * pass_bytes(live);
+            const int tokens_end = last_unit + kPowerBytes + kTokens * kTokenBytes;
+            if (tokens_end > ring(live) || kExchange > ring(live) || ring(live) % 16 ||
+                shared(live) > shared(kTokens) || shared(live) > 227 * 1024)
+                return false;
+        }
+        return true;
+    }
     static int resident(int live)
     {
         const int fit = 228 * 1024 / (shared(live) + 1024);
@@ -592,6 +606,7 @@ template <int Columns, int Group, typename Scale, bool Zeros>
 cudaError_t launch_kernel(camblas_cuda_context *context, LinearTask task)
 {
     typedef Stage<Columns, Group, Scale, Zeros> S;
+    static_assert(S::reads_inside(), "shared memory of a stage");
     const int blocks = (task.outputs + kWarps * 16 - 1) / (kWarps * 16);
     const int passes = (task.rows + S::kTokens - 1) / S::kTokens;
     const int live = task.rows < S::kTokens ? task.rows : S::kTokens;
