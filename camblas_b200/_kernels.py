@@ -15,6 +15,7 @@ import ctypes as ct
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._native import algorithm, kernel_family, set_algorithm, stats  # noqa: F401
@@ -741,6 +742,7 @@ def reduce_groups(grouped, experts, reverse):
 
 
 _NO_GRADIENT = "An operand requires a gradient: this operation has none, call it under torch.no_grad()"
+_NO_TANGENT = "An operand carries a forward-mode gradient: this operation has none"
 
 
 def _refuse_gradient(*tensors):
@@ -748,6 +750,10 @@ def _refuse_gradient(*tensors):
     for tensor in tensors:
         if tensor is not None and tensor.requires_grad and torch.is_grad_enabled():
             raise ValueError(_NO_GRADIENT)
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # inside a dual level, the only place where tangents live
+        for tensor in tensors:
+            if tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None:
+                raise ValueError(_NO_TANGENT)
 
 
 def _address(tensor):
