@@ -9,7 +9,8 @@
  * p of a table the caller computed (angles of far positions lose their
  * fraction in FP32, so they are not formed here). Everything between the load
  * and the store is FP32; the result, divided by the scale of its cache, is rounded
- * once, to BF16 or, for an 8-bit cache, from FP32 straight to E4M3.
+ * once, to BF16 or, for an 8-bit cache, from FP32 straight to E4M3. A head whose
+ * squares leave FP32's range is done again, divided by a power of two.
  *
  * The reads and writes of the heads bound the kernel: seven operations per
  * element against four bytes, as long as issue keeps up: a head's eight elements
@@ -30,6 +31,7 @@
 
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace heads
 {
@@ -202,6 +204,49 @@ template <bool Interleaved> struct Turn {
     }
 };
 
+/* Bits of 2^-90 and 2^120: means of squares between them are of squares that FP32 holds. */
+constexpr unsigned kLeastMean = (127 - 90) << 23, kMostMean = (127 + 120) << 23;
+
+/* The norm's factor of a head whose squares leave FP32's range or its normal numbers: from squares of the
+ * elements divided by the power of two of the largest, or of the root of epsilon where that is larger, which
+ * `x` then is too. A head of zeros, or with an element that is not finite, keeps the factor it has. */
+template <int Lanes>
+__device__ __forceinline__ float far_scale(unsigned sharing, Eight &x, float scale, float inverse_depth, float epsilon)
+{
+    float largest = 0.f;
+    bool broken = false;
+    const Two parts[4] = {x.a[0], x.a[1], x.b[0], x.b[1]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = both(parts[i]);
+        largest = fmaxf(largest, fmaxf(fabsf(v.x), fabsf(v.y)));
+        broken = broken || !(fabsf(v.x) < INFINITY) || !(fabsf(v.y) < INFINITY);
+    }
+#pragma unroll
+    for (int offset = Lanes / 2; offset > 0; offset /= 2)
+        largest = fmaxf(largest, __shfl_xor_sync(sharing, largest, offset, Lanes));
+    if (__any_sync(sharing, broken) || largest == 0.f)
+        return scale;
+    int exponent = ilogbf(largest);
+    if (epsilon > 0.f)
+        exponent = max(exponent, ilogbf(epsilon) / 2);
+    const float down = ldexpf(1.f, -exponent / 2), rest = ldexpf(1.f, -exponent - -exponent / 2);
+    float square = 0.f;
+    Eight y = x;
+    Two *const out[4] = {&y.a[0], &y.a[1], &y.b[0], &y.b[1]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        *out[i] = multiply(multiply(parts[i], two(down, down)), two(rest, rest));
+        const float2 v = both(*out[i]);
+        square += v.x * v.x + v.y * v.y;
+    }
+#pragma unroll
+    for (int offset = Lanes / 2; offset > 0; offset /= 2)
+        square += __shfl_xor_sync(sharing, square, offset, Lanes);
+    x = y;
+    return rsqrtf(square * inverse_depth + epsilon * down * rest * down * rest);
+}
+
 /* `Lanes` lanes share a head; a CTA takes one token's query heads, key heads and,
  * with a cache, value heads, or every gridDim.y-th round of them. What does not
  * depend on the head (the products of weight and cosine or sine) is done once
@@ -225,16 +270,19 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
     const float *cosines = task.table + position * task.rotary + 4 * unit;
 
     /* Works on heads h = begin, begin + step, ... below count, the first at `source`: turns them
-     * (nullptr: leaves them as they are) and hands each to store(h, a, b). */
+     * (nullptr: leaves them as they are) and hands each to store(h, a, b). Returns whether a norm left
+     * the range, and the heads are to be done again with `careful`. */
     const auto run = [&](int begin, int count, const __nv_bfloat16 *source, int head_stride, const auto *turn,
-                         bool normalise, auto store) {
+                         bool normalise, auto store, auto careful) {
+        constexpr int kAtOnce = careful.value ? 1 : Batch;
+        bool far = false;
         const __nv_bfloat16 *at_first = source + (long long)begin * head_stride + first;
         const __nv_bfloat16 *at_second = at_first + (second - first);
         const long long ahead = (long long)step * head_stride;
-        for (int head = begin; head < count; head += Batch * step) {
-            uint2 raw[Batch][2];
+        for (int head = begin; head < count; head += kAtOnce * step) {
+            uint2 raw[kAtOnce][2];
 #pragma unroll
-            for (int i = 0; i < Batch; ++i) {
+            for (int i = 0; i < kAtOnce; ++i) {
                 raw[i][0] = raw[i][1] = make_uint2(0, 0);
                 if (live && head + i * step < count) {
                     raw[i][0] = *reinterpret_cast<const uint2 *>(at_first);
@@ -243,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
                 at_first += ahead, at_second += ahead;
             }
 #pragma unroll
-            for (int i = 0; i < Batch; ++i) {
+            for (int i = 0; i < kAtOnce; ++i) {
                 if (head + i * step >= count)
                     break;
                 Eight x = {{widen_pair(raw[i][0].x), widen_pair(raw[i][0].y)},
@@ -258,7 +306,16 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
 #pragma unroll
                         for (int offset = Lanes / 2; offset > 0; offset /= 2)
                             square += __shfl_xor_sync(sharing, square, offset, Lanes);
-                        scale = rsqrtf(square * task.inverse_depth + task.epsilon);
+                        const float mean = square * task.inverse_depth + task.epsilon;
+                        scale = rsqrtf(mean);
+                        /* the same for all lanes of the head; a NaN is outside too */
+                        const bool outside = __float_as_uint(mean) - kLeastMean >= kMostMean - kLeastMean;
+                        if constexpr (careful.value) {
+                            if (outside)
+                                scale = far_scale<Lanes>(sharing, x, scale, task.inverse_depth, task.epsilon);
+                        } else {
+                            far = far || outside;
+                        }
                     }
                     x = turn->apply(x, turns, scale);
                 }
@@ -266,6 +323,14 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
                     store(head + i * step, as_piece(x.a), as_piece(x.b));
             }
         }
+        return far;
+    };
+    /* The careful loop stands apart: its code within the other's takes registers that the heads in flight
+     * need (8192 tokens: 61.7 us, apart 60.3). */
+    const auto run_normed = [&](int begin, int count, const __nv_bfloat16 *source, int head_stride, const auto *turn,
+                                bool normalise, auto store) {
+        if (run(begin, count, source, head_stride, turn, normalise, store, std::false_type{}))
+            run(begin, count, source, head_stride, turn, normalise, store, std::true_type{});
     };
 
     if (!placed) { /* a padding row: zeros, and nothing enters the cache */
@@ -284,7 +349,8 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
         const Turn<Interleaved> turn(live ? task.q_weight : nullptr, cosines, task.rotary / 2, turns, first,
                                      second);
         __nv_bfloat16 *out = task.q_out + (long long)token * task.heads * task.depth;
-        run(group, task.heads, task.q + token * task.q_token, task.q_head, &turn, task.q_weight != nullptr,
+        run_normed(
+            group, task.heads, task.q + token * task.q_token, task.q_head, &turn, task.q_weight != nullptr,
             [&](int head, const Piece &a, const Piece &b) {
                 store_piece(out + head * task.depth + first, a), store_piece(out + head * task.depth + second, b);
             });
@@ -320,7 +386,8 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
                                      second);
         __nv_bfloat16 *out =
             task.k_out ? task.k_out + (long long)token * task.kv_heads * task.depth : nullptr;
-        run(begin, task.kv_heads, task.k + token * task.k_token, task.k_head, &turn, task.k_weight != nullptr,
+        run_normed(
+            begin, task.kv_heads, task.k + token * task.k_token, task.k_head, &turn, task.k_weight != nullptr,
             [&](int head, const Piece &a, const Piece &b) {
                 if (out)
                     store_piece(out + head * task.depth + first, a), store_piece(out + head * task.depth + second, b);
@@ -329,9 +396,11 @@ __global__ void __launch_bounds__(kThreads, Batch > 1 ? 16 : 1) rotate_kernel(co
     }
     begin = first_after(task.heads + task.kv_heads);
     if (task.v && begin < task.kv_heads && page >= 0)
-        run(begin, task.kv_heads, task.v + token * task.v_token, task.v_head,
+        run(
+            begin, task.kv_heads, task.v + token * task.v_token, task.v_head,
             static_cast<const Turn<Interleaved> *>(nullptr), false,
-            [&](int head, const Piece &a, const Piece &b) { cache(task.value_cache, head, task.value_scale, a, b); });
+            [&](int head, const Piece &a, const Piece &b) { cache(task.value_cache, head, task.value_scale, a, b); },
+            std::false_type{});
 }
 
 template <int Lanes, int Batch> void launch_batch(camblas_cuda_context *context, const RotateTask &task, int parts)

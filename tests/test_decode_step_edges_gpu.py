@@ -224,3 +224,24 @@ def test_int4_codes_at_and_near_the_zero_point(gen, rows, group, zeros):
     out = _kernels.int4_linear(x, weight)
     assert not out[:, :50].any()
     assert exact.within(out, *exact.int4(x, codes, scale, zero))
+
+
+@pytest.mark.parametrize("depth,rotary,interleaved", [(64, 64, False), (128, 64, True), (256, 256, False), (8, 8, True)])
+def test_norm_of_heads_whose_squares_leave_the_range(gen, depth, rotary, interleaved):
+    """Squares beyond FP32's largest number, and below its smallest ones where epsilon does not cover them."""
+    sizes = (2.0 ** 62, 2.0 ** 90, 2.0 ** 125, 2.0 ** -66, 2.0 ** -90, 2.0 ** -118, 1.0)
+    x = normal(gen, len(sizes), 3, depth)
+    x = (x.clamp(-3, 3) * torch.tensor(sizes, device="cuda")[:, None, None]).to(BF16)
+    x[2, 0] = torch.finfo(BF16).max
+    w = (1 + 0.3 * normal(gen, depth)).to(BF16)
+    table = _kernels.rotary_table(512, rotary)
+    positions = integers(gen, 0, 512, len(sizes))
+    for epsilon in (0.0, 1e-6):
+        q_out, k_out = _kernels.qk_norm_rope(x, x[:, :1], w, w, epsilon, positions, table, interleaved=interleaved)
+        want, bound = exact.norm_rope(x, w, epsilon, positions, table, interleaved)
+        assert exact.within(q_out, want, bound)
+        assert torch.equal(q_out[:, :1], k_out)
+    zero = torch.zeros(1, 1, depth, device="cuda", dtype=BF16)
+    assert not _kernels.qk_norm_rope(zero, zero, w, w, 1e-30, positions[:1], table)[0].any()
+    zero[0, 0, 3] = float("inf")
+    assert _kernels.qk_norm_rope(zero, zero, None, None, 1e-6, positions[:1] * 0, table)[0][0, 0, 3].isinf()
