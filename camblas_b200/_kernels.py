@@ -938,6 +938,10 @@ def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, windo
         raise ValueError("lengths must be contiguous CUDA int32 [batch]")
     if not 0 <= window <= _INT_MAX or not 0 <= sinks <= _INT_MAX:
         raise ValueError("window and sinks must not be negative")
+    if scale is None:
+        scale = depth ** -0.5
+    if not (abs(scale) < _INFINITY and abs(key_scale) < _INFINITY and abs(value_scale) < _INFINITY):
+        raise ValueError("scales must be finite")
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if batch:
         native = _native.context(index)
@@ -945,8 +949,7 @@ def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, windo
                                       window, sinks)
         # of the calling stream's pool, or of the capturing graph's own: no other call shares it
         workspace = q.new_empty((size // 2,))
-        native.call("paged_attention", batch, heads, kv_heads, depth, depth ** -0.5 if scale is None else scale,
-                    q.data_ptr(), code, key_cache.data_ptr(), value_cache.data_ptr(),
+        native.call("paged_attention", batch, heads, kv_heads, depth, scale, q.data_ptr(), code, key_cache.data_ptr(), value_cache.data_ptr(),
                     _stride_array(q_row, q_head, *strides, row), pages, page_size, key_scale, value_scale,
                     table.data_ptr(), width, lengths.data_ptr(), window, sinks, workspace.data_ptr(), size,
                     out.data_ptr())
@@ -1072,6 +1075,7 @@ def route_experts(logits, choices, bias=None, scoring="softmax", groups=1, kept_
              "route_experts takes up to 1024 experts in up to 32 equal groups and up to 32 choices among the kept")
     _require(bias is None or (bias.get_device() == index and bias.dtype is torch.float32 and bias.shape == (experts,)
                               and bias.is_contiguous()), "bias must be contiguous CUDA FP32 [experts]")
+    _require(abs(scale) < _INFINITY, "scale must be finite")
     row, unit = logits.stride()
     if unit != 1 or (tokens > 1 and row < experts):
         logits = logits.contiguous()

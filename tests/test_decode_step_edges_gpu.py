@@ -245,3 +245,14 @@ def test_norm_of_heads_whose_squares_leave_the_range(gen, depth, rotary, interle
     assert not _kernels.qk_norm_rope(zero, zero, w, w, 1e-30, positions[:1], table)[0].any()
     zero[0, 0, 3] = float("inf")
     assert _kernels.qk_norm_rope(zero, zero, None, None, 1e-6, positions[:1] * 0, table)[0][0, 0, 3].isinf()
+
+
+def test_scales_that_are_not_finite_are_refused(gen):
+    keys, values, table, counts = paged(gen, (30,), 16, 2, 64)
+    q = normal(gen, 1, 4, 64).to(BF16)
+    for name in ("scale", "key_scale", "value_scale"):
+        for value in (float("nan"), float("inf"), -float("inf")):
+            with pytest.raises(ValueError):
+                _kernels.paged_attention(q, keys, values, table, counts, **{name: value})
+            with pytest.raises(ValueError):
+                _kernels.route_experts(normal(gen, 2, 8), 2, scale=value)
