@@ -949,7 +949,8 @@ def paged_attention(q, key_cache, value_cache, table, lengths, scale=None, windo
                                       window, sinks)
         # of the calling stream's pool, or of the capturing graph's own: no other call shares it
         workspace = q.new_empty((size // 2,))
-        native.call("paged_attention", batch, heads, kv_heads, depth, scale, q.data_ptr(), code, key_cache.data_ptr(), value_cache.data_ptr(),
+        native.call("paged_attention", batch, heads, kv_heads, depth, scale, q.data_ptr(), code,
+                    key_cache.data_ptr(), value_cache.data_ptr(),
                     _stride_array(q_row, q_head, *strides, row), pages, page_size, key_scale, value_scale,
                     table.data_ptr(), width, lengths.data_ptr(), window, sinks, workspace.data_ptr(), size,
                     out.data_ptr())

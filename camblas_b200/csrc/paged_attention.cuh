@@ -21,13 +21,13 @@
  * want 128 rows of M and bring nothing to a kernel that waits for HBM; mma.sync
  * does a product in 8 cycles per sub-core here, a quarter of the time that HBM
  * gives.) Scores, statistics, sums and the joined result are FP32; P goes to the
- * value product in two parts, rounded to BF16 and what that leaves, rounded again
- * (over an 8-bit cache FP16): at most 2^-16 (2^-22) of each weight is lost. In one
- * part the 2^-8 (2^-11) of each weight made the result's error against 64 bits 3 to
- * 13 % larger than its last rounding alone. FP16 keeps its bits only down to 2^-14,
- * and a result can be made of weights far below the largest (a first token that
- * takes the weight and has next to no value), so over an 8-bit cache P is 2^15 times
- * the weights, and what lies below 2^-40 of the largest is lost.
+ * value product in two parts, of BF16 the upper half and what that leaves, rounded
+ * (over an 8-bit cache FP16, both rounded): at most 2^-16 (2^-22) of each weight is
+ * lost. In one part the 2^-8 (2^-11) of each weight made the result's error against
+ * 64 bits 3 to 13 % larger than its last rounding alone. FP16 keeps its bits only
+ * down to 2^-14, and a result can be made of weights far below the largest (a first
+ * token that takes the weight and has next to no value), so over an 8-bit cache P is
+ * 2^15 times the weights, and what lies below 2^-40 of the largest is lost.
  *
  * Measured, 64 query and 8 key heads of 128 in BF16: one sequence of 130977
  * tokens 98 us (0.84 of the measured copy rate), 48 sequences of 0 to 8191 tokens
@@ -294,12 +294,25 @@ template <bool Half> __device__ __forceinline__ uint32_t pack(float low, float h
     }
 }
 
-template <bool Half> __device__ __forceinline__ float2 unpack(uint32_t raw)
+/* Two weights as the sums of two 16-bit parts each. A BF16 value may be infinite, and its weight's parts
+ * have to be positive then: the first part is cut off, not rounded, and the rest is 2^-17 of the weight at
+ * least. (E4M3 has no infinities.) */
+struct Parts {
+    uint32_t first, rest;
+};
+
+template <bool Half> __device__ __forceinline__ Parts in_parts(float low, float high)
 {
-    if constexpr (Half)
-        return __half22float2(*reinterpret_cast<const __half2 *>(&raw));
-    else
-        return make_float2(__uint_as_float(raw << 16), __uint_as_float(raw & 0xffff0000u));
+    if constexpr (Half) {
+        const uint32_t first = pack<true>(low, high);
+        const float2 taken = __half22float2(*reinterpret_cast<const __half2 *>(&first));
+        return {first, pack<true>(low - taken.x, high - taken.y)};
+    } else {
+        const float low_rest = low - __uint_as_float(__float_as_uint(low) & 0xffff0000u);
+        const float high_rest = high - __uint_as_float(__float_as_uint(high) & 0xffff0000u);
+        return {__byte_perm(__float_as_uint(low), __float_as_uint(high), 0x7632),
+                pack<false>(fmaxf(low_rest, low * 0x1p-17f), fmaxf(high_rest, high * 0x1p-17f))};
+    }
 }
 
 /* 2^x; 0 for -infinity */
@@ -647,11 +660,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<Depth, Blocks, Eight>::kRes
                     constexpr float kFactor = Eight ? kRaised : 1.f;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float low = score[m][2 * i] * kFactor, high = score[m][2 * i + 1] * kFactor;
-                        const uint32_t rounded = pack<Eight>(low, high);
-                        const float2 taken = unpack<Eight>(rounded);
-                        p[n][m][i] = transpose_8x8(rounded);
-                        rest[n][m][i] = transpose_8x8(pack<Eight>(low - taken.x, high - taken.y));
+                        const Parts parts =
+                            in_parts<Eight>(score[m][2 * i] * kFactor, score[m][2 * i + 1] * kFactor);
+                        p[n][m][i] = transpose_8x8(parts.first), rest[n][m][i] = transpose_8x8(parts.rest);
                     }
                 }
             }

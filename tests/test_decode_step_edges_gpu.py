@@ -64,6 +64,22 @@ def test_weights_keep_more_bits_than_the_values(gen, kind, heads, depth, length)
     assert exact.within(out, want, bound)
 
 
+@pytest.mark.parametrize("heads,depth", [(1, 64), (16, 128), (3, 256)])
+def test_infinite_values_stay_infinite(gen, heads, depth):
+    """A visible infinity has a positive weight: its column is infinite in its sign, and the others are finite."""
+    keys, values, table, counts = paged(gen, (1, 150, 700), 16, 1, depth)
+    q = normal(gen, 3, heads, depth).to(BF16)
+    q[2] = 0  # weights that are powers of two, which a first part holds whole
+    for b, t in ((0, 0), (1, 149), (2, 333)):
+        row = values[int(table[b, t // 16]), t % 16, 0]
+        row[3], row[depth - 1] = float("inf"), -float("inf")
+    out = _kernels.paged_attention(q, keys, values, table, counts)
+    assert (out[..., 3] == float("inf")).all() and (out[..., depth - 1] == -float("inf")).all()
+    rest = torch.ones(depth, dtype=torch.bool, device="cuda")
+    rest[3] = rest[depth - 1] = False
+    assert out[..., rest].isfinite().all()
+
+
 def attention_by_c(gen, batch=2, offset=0):
     """Status, message and output of a small call through the C ABI, the output `offset` elements into its buffer."""
     keys, values, table, counts = paged(gen, (30, 20), 16, 2, 64)
