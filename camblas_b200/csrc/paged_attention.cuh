@@ -295,7 +295,7 @@ template <bool Half> __device__ __forceinline__ uint32_t pack(float low, float h
 }
 
 /* Two weights as the sums of two 16-bit parts each. A BF16 value may be infinite, and its weight's parts
- * have to be positive then: the first part is cut off, not rounded, and the rest is 2^-17 of the weight at
+ * have to be positive then: the first part is cut off, not rounded, and the rest is 2^-24 of the weight at
  * least. (E4M3 has no infinities.) */
 struct Parts {
     uint32_t first, rest;
@@ -311,7 +311,7 @@ template <bool Half> __device__ __forceinline__ Parts in_parts(float low, float 
         const float low_rest = low - __uint_as_float(__float_as_uint(low) & 0xffff0000u);
         const float high_rest = high - __uint_as_float(__float_as_uint(high) & 0xffff0000u);
         return {__byte_perm(__float_as_uint(low), __float_as_uint(high), 0x7632),
-                pack<false>(fmaxf(low_rest, low * 0x1p-17f), fmaxf(high_rest, high * 0x1p-17f))};
+                pack<false>(fmaxf(low_rest, low * 0x1p-24f), fmaxf(high_rest, high * 0x1p-24f))};
     }
 }
 
