@@ -22,10 +22,10 @@
  *
  * One warp per token, expert e on lane e % 32; a round of the choice is a local
  * maximum and two warp reductions of 32-bit keys that are ordered like the ranks.
- * Issue bounds the kernel, not its few bytes per token: some 670 instructions for
- * a token's eight of 128 experts, 16384 tokens in 14.7 us (28 with FP64 ranks for
- * all); one token among 256 experts in eight groups takes 7.4 us, the latency of
- * its chain of reductions.
+ * Issue bounds the kernel, not its few bytes per token: some 700 instructions for
+ * a token's eight of 128 experts, 16384 tokens in 14.9 us (28 with FP64 ranks for
+ * all), 62 us with a bias and eight of 256 experts in eight groups; one token among
+ * those takes 7.0 us, the latency of its chain of reductions.
  */
 #pragma once
 

@@ -14,9 +14,9 @@
  *
  * The reads and writes of the heads bound the kernel: seven operations per
  * element against four bytes, as long as issue keeps up: a head's eight elements
- * of a lane take about 130 instructions here; the first form, which divided by
+ * of a lane take about 140 instructions here; the first form, which divided by
  * the heads per token and multiplied weight, cosine and sine for every head, took
- * 250 and 117 us where this takes 60 (8192 tokens of 64 + 8 heads of 128; 0.78 of
+ * 250 and 117 us where this takes 60 (8192 tokens of 64 + 8 heads of 128; 0.77 of
  * the measured copy rate). As many lanes as a depth needs at eight elements per
  * lane, rounded up to a power of two, share a head; a lane holds both members of
  * its pairs, so the rotation needs no exchange and the norm one shuffle tree. A

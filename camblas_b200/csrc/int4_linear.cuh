@@ -583,8 +583,8 @@ __global__ void __launch_bounds__(kWarps * 32, 7) few_kernel(const __grid_consta
  * model of the time: a CTA alone on an SM takes `alone` for a unit, k CTAs
  * together `shared` each (what HBM gives an SM, or the products of the columns),
  * and CTAs that do not fit wait. Measured (37 tokens, 7168 -> 4992, groups of
- * 128): 23.6, 22.8, 23.1, 23.6 and 23.2 us with 1, 2, 3, 4 and 7 ranges, the
- * chosen one 22.2; 64 outputs alone would leave 147 SMs without work. */
+ * 128): 39.8, 30.9, 22.9, 21.2 and 24.9 us with 1, 2, 3, 4 and 7 ranges, the
+ * chosen number 20.4; 64 outputs alone would leave 147 SMs without work. */
 inline int choose_split(int blocks, int units, int step, int columns, int sm_count, int resident)
 {
     const double alone = 0.15 + 0.06 * columns, shared = 0.05 * columns > 0.1 ? 0.05 * columns : 0.1;
@@ -705,9 +705,16 @@ inline int prepare_kernels()
 template <int Group, typename Scale>
 cudaError_t launch_rows(camblas_cuda_context *context, const LinearTask &task, bool zeros)
 {
-    /* few_kernel while one wave of its CTAs has a place for every tile of outputs; with more, the
-     * block kernel keeps its ring full where few_kernel would start anew (one token, 8192 -> 28672:
-     * 50 us by few_kernel, 40 by the block kernel; 28672 -> 8192: 30 and 42) */
+    /* few_kernel while one wave of its CTAs has a place for every tile of outputs (16576 outputs); with
+     * more, the block kernel keeps its ring full where few_kernel would start anew. One token, groups of
+     * 128, few_kernel and block kernel in us:
+     *   outputs            8192        12288       16384       18432       20480       24576       28672
+     *   4096 inputs     8.4   8.9   10.1  10.9  11.4  15.7  18.1  14.2  18.7  18.5  20.7  17.0  18.1  23.5
+     *   8192 inputs    12.4  16.9   24.6  19.2  18.1  23.7  37.6  22.8  37.0  27.7  31.4  32.1  48.7  41.4
+     *   16384 inputs   19.5  25.1   37.0  31.4  31.4  37.9  67.1  36.7  56.1  43.6  52.6  50.4  74.5  63.6
+     * and the same order with two, four and eight, except where they are within a tenth. The rule is wrong
+     * at 12288 outputs of wide inputs, whose split few_kernel chooses over several waves, and at 28672
+     * outputs of 4096 inputs. */
     if (task.rows <= 8)
         return (task.outputs + 15) / 16 <= 7ll * context->sm_count ? launch_few<Group, Scale>(context, task, zeros)
                                                                    : launch<1, Group, Scale>(context, task, zeros);

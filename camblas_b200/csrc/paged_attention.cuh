@@ -19,8 +19,8 @@
  * that hold the head's column in both products. P^T turns from the accumulator's
  * to the operand's layout by movmatrix, without shared memory. (tcgen05 would
  * want 128 rows of M and bring nothing to a kernel that waits for HBM; mma.sync
- * does a product in 8 cycles per sub-core here, a quarter of the time that HBM
- * gives.) Scores, statistics, sums and the joined result are FP32; P goes to the
+ * does a product in 8 cycles per sub-core here, the 24 of 16 tokens of 128 columns
+ * in a seventh of the time that HBM gives.) Scores, statistics, sums and the joined result are FP32; P goes to the
  * value product in two parts, of BF16 the upper half and what that leaves, rounded
  * (over an 8-bit cache FP16, both rounded): at most 2^-16 (2^-22) of each weight is
  * lost. In one part the 2^-8 (2^-11) of each weight made the result's error against
@@ -30,9 +30,10 @@
  * 2^15 times the weights, and what lies below 2^-40 of the largest is lost.
  *
  * Measured, 64 query and 8 key heads of 128 in BF16: one sequence of 130977
- * tokens 98 us (0.84 of the measured copy rate), 48 sequences of 0 to 8191 tokens
+ * tokens 98 us (0.83 of the measured copy rate), 48 sequences of 0 to 8191 tokens
  * 60 us (0.61; some 5 us are the way from the lengths to the first keys, and 11
- * the join), one of 300 tokens 9.5 us.
+ * the join), one of 300 tokens 9.6 us. Over an 8-bit cache widening to FP16 and the
+ * products of the weights' second part show: 69 and 50 us, 0.59 and 0.37.
  *
  * Work split. A warp works alone. The slots of a sequence (key heads times
  * blocks of 8 or 16 query heads) are taken in teams of four neighbours, two or
@@ -364,9 +365,9 @@ template <int Depth, int Blocks, bool Eight> struct Shape {
     static constexpr int kTileBytes = 2 * kTile * kRowBytes; /* keys and values */
     /* The copies in flight on an SM have to cover the latency of HBM at its share of the bandwidth,
      * some 45 KB. Two stages do, and let more warps share the SM (48 ragged sequences of 128 BF16
-     * columns: 60 us, three stages 65), unless registers keep the third CTA away or make it spill:
-     * sixteen heads at 128 BF16 columns (eight sequences, one key head: 28 us with three, 34 with
-     * two). */
+     * columns: 60 us, three stages 64), unless registers keep the third CTA away or make it spill:
+     * sixteen heads at 128 BF16 columns (eight sequences, one key head: 28.5 us with three, 34.4 with
+     * two). At 256 BF16 columns three are within 5 % of two (sixteen sequences: 31.5 and 29.9). */
     static constexpr int kStages = kRowBytes >= 512 || (kRowBytes == 256 && Blocks == 2) ? 3 : 2;
     static constexpr int kNoteBytes = 16 * kTile + 16; /* where the rows of a stage lie, which are real */
     static constexpr int kWarpBytes = kStages * (kTileBytes + kNoteBytes);
