@@ -13,12 +13,13 @@
  * Which expert is chosen is a whole number that no tolerance covers, and ranks
  * may lie closer than FP32 can tell: they are compared in FP64. Without bias and
  * groups the choice is made on the logits themselves, with which both scores grow;
- * otherwise on FP32 ranks, whose error is bounded. It is made again on FP64 ranks for a
- * token where two ranks that decide anything lie within that bound (a few
+ * otherwise on FP32 ranks, whose error is bounded. It is made again on FP64 ranks
+ * for a token where two ranks that decide anything lie within that bound (a few
  * tokens in a thousand; every FP64 exponential costs some forty instructions of a
  * rate of one in two), or where distinct logits that decide anything may have one
- * FP64 score (saturated sigmoids, exponentials that underflow). The weights are FP64 throughout, which is cheap for the
- * chosen few: renormalised softmax weights do not need the sum over all.
+ * FP64 score (saturated sigmoids, exponentials that underflow). The weights are
+ * FP64 throughout, which is cheap for the chosen few: renormalised softmax weights
+ * do not need the sum over all.
  *
  * One warp per token, expert e on lane e % 32; a round of the choice is a local
  * maximum and two warp reductions of 32-bit keys that are ordered like the ranks.
@@ -232,8 +233,8 @@ __device__ __forceinline__ float group_doubt(float magnitude) { return 0x1p-17f 
 
 /* Whether the scores of two logits, the larger first, are in the same order in FP64, and equal only where
  * the logits are. From 2^-25 apart the exponentials differ by that relative to them, and by far more than
- * FP64 rounds off, as long as the larger score is a normal number (`base` is the
- * largest logit, for a sigmoid 0) and the 1 that a sigmoid adds to its exponential does not cover it. */
+ * FP64 rounds off, as long as the larger score is a normal number (`base` is the largest logit, for a sigmoid
+ * 0) and the 1 that a sigmoid adds to its exponential does not cover the difference. */
 __device__ __forceinline__ bool scores_ordered(float larger, float smaller, float base, bool sigmoid)
 {
     return larger == smaller || (larger - smaller > 0x1p-25f && larger - base > -700.f && !(sigmoid && larger > 16.f));
